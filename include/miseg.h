@@ -52,6 +52,7 @@ extern "C" {
 #define MISEG_ACT_RELU 1
 #define MISEG_ACT_SOFTMAX 2 /* over Cout (<= 4), fp32 output, optional u8 collapse */
 #define MISEG_ACT_SIGMOID 3
+#define MISEG_ACT_SILU 4 /* z * sigmoid(z); the group-normalisation and checkpoint entry points */
 
 #define MISEG_CONV_DGRAD_T 2 /* miseg_conv_desc.transposed: data gradient of the transpose convolution */
 #define MISEG_TILE_NO_DMA 16
@@ -534,6 +535,108 @@ int miseg_bn_relu_bwd_apply(const void* x, const void* dy, void* dx, int64_t pix
  * Pass 2 then runs with relu = 0 on the stored g. */
 int miseg_bn_bwd_sums(const double* stats, int32_t replicas, int32_t stride, int32_t C, const float* mean,
                       const float* var, float eps, double* sums, void* stream);
+
+/*
+ * Group normalisation with an activation, channels last (keras GroupNormalization + Activation; the reference builds
+ * BatchNormalization only, utils/model.py:176-211: this is the form for batches too small for batch statistics).
+ * x: N images of `pixels` pixels with C channels, in `groups` groups of w = C / groups consecutive channels; m = pixels * w.
+ *   mean[n][g] = sum x / m;  rstd[n][g] = 1 / sqrt(sum (x - mean)^2 / m + eps)
+ *   scale[n][c] = gamma[c] * rstd;  shift[n][c] = beta[c] - mean * scale       (gamma NULL: 1, beta NULL: 0)
+ *   y = act(x * scale + shift)
+ * groups = C is instance normalisation; N = 1 with all pixels of a batch and groups = C is BatchNormalization on batch
+ * statistics.  mean, rstd, scale and shift are outputs that the backward call takes.
+ * codes, code_scales (both or neither): the 8-bit checkpoint of xhat = (x - mean) * rstd, written in the same pass.
+ *
+ * Tensors: dtype MISEG_DT_BF16 (16 bits in format fmt) or MISEG_DT_F32; `*_pix` / `*_img` are the strides of a pixel and of
+ * an image in elements, so a tensor can be a channel slice of a wider buffer; pointers and strides are multiples of 16
+ * bytes, C of 8.  y may be x itself or another channel range of x's buffer and overlaps it in no other way.  Statistics
+ * and sums are in fp32 per thread and fp64 across threads, without atomics: equal calls give equal bits.  Results are
+ * rounded once; what exceeds the range of fp16 becomes an infinity.
+ * workspace: miseg_group_norm_workspace(N, pixels, C, backward) bytes, 16-byte aligned, not cleared by anyone; calls that
+ * overlap in time need one each.
+ */
+typedef struct miseg_group_norm_desc {
+  const void* x;
+  void* y;
+  const float* gamma;
+  const float* beta;
+  float* mean;
+  float* rstd;
+  float* scale;
+  float* shift;
+  int8_t* codes;
+  uint16_t* code_scales;
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t pixels;
+  int64_t x_img, y_img;
+  int32_t x_pix, y_pix;
+  int32_t N, C, groups;
+  int32_t dtype, fmt, act;
+  float eps;
+} miseg_group_norm_desc;
+int64_t miseg_group_norm_workspace(int32_t N, int64_t pixels, int32_t C, int32_t backward);
+int miseg_group_norm_act_fwd(const miseg_group_norm_desc* d, void* stream);
+
+/*
+ * Its backward pass, from x or from the checkpoint of xhat (codes and code_scales; x NULL).
+ *   g = dy * act'(z), z = x * scale + shift (checkpoint: xhat * gamma + beta)
+ *   dbeta[c] = sum g;  dgamma[c] = sum g * xhat                                (either may be NULL)
+ *   dx = scale * g - sum_group(scale * sum g) / m - xhat * sum_group(scale * sum g * xhat) / m
+ * mean, rstd, scale, shift: of the forward call.  dx may be x or dy itself (or another channel range of their buffers).
+ */
+typedef struct miseg_group_norm_bwd_desc {
+  const void* x;
+  const int8_t* codes;
+  const uint16_t* code_scales;
+  const void* dy;
+  void* dx;
+  const float* mean;
+  const float* rstd;
+  const float* scale;
+  const float* shift;
+  const float* gamma;
+  const float* beta;
+  float* dgamma;
+  float* dbeta;
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t pixels;
+  int64_t x_img, dy_img, dx_img;
+  int32_t x_pix, dy_pix, dx_pix;
+  int32_t N, C, groups;
+  int32_t dtype, fmt, act;
+} miseg_group_norm_bwd_desc;
+int miseg_group_norm_act_bwd(const miseg_group_norm_bwd_desc* d, void* stream);
+
+/*
+ * Activation checkpoints in 8 bits: codes int8 [N * pixels][C], code_scales bf16 [N * pixels][ceil(C / 32)], dense.  32
+ * consecutive channels of a pixel share code_scale = bf16(max |v| / 127); v is read back as code * code_scale.  A block
+ * whose largest magnitude is below 2^-119 is zero; a block that holds an infinity or a NaN reads back as NaN.
+ * Write: v = x * code_a[c] + code_b[c], or x where code_a is NULL; with y also y = act(x * y_a[c] + y_b[c]) in the same
+ * pass (a normalisation layer's apply pass that leaves its checkpoint behind).
+ * Read: y = act(v * y_a[c] + y_b[c]), or act(v) where y_a is NULL: the operand of a weight gradient.
+ * Coefficients are fp32, 16-byte aligned, coef_img elements (0: the same ones, else a multiple of 4) from one image's to
+ * the next's.  Strides, types and overlap as in miseg_group_norm_desc.
+ */
+typedef struct miseg_checkpoint8_desc {
+  const void* x;               /* write */
+  void* y;                     /* read; optional in write */
+  int8_t* codes;
+  uint16_t* code_scales;
+  const float* code_a;         /* write */
+  const float* code_b;
+  const float* y_a;
+  const float* y_b;
+  int64_t pixels;
+  int64_t x_img, y_img;
+  int64_t coef_img;
+  int32_t x_pix, y_pix;
+  int32_t N, C;
+  int32_t dtype, fmt, act;
+} miseg_checkpoint8_desc;
+int miseg_checkpoint8_write(const miseg_checkpoint8_desc* d, void* stream);
+int miseg_checkpoint8_read(const miseg_checkpoint8_desc* d, void* stream);
 
 /* dx of ZeroPadding2D(1)+MaxPooling2D(3,2): the gradient goes to the first maximum of each
  * window in row-major scan order.  x: pool input [N,H,W,C], dy: [N,H/2,W/2,C], bf16.  addend (may be NULL):

@@ -41,6 +41,11 @@ int launch_bn_relu_bwd_apply(const void*, const void*, void*, long long, int, in
                              const double*, const void*, int, hipStream_t);
 int launch_bn_bwd_sums(const double*, int, int, int, const float*, const float*, float, double*, hipStream_t);
 int launch_channel_sums(const void*, long long, int, int, double*, hipStream_t);
+int launch_group_norm_fwd(const miseg_group_norm_desc*, hipStream_t);
+int launch_group_norm_bwd(const miseg_group_norm_bwd_desc*, hipStream_t);
+int launch_checkpoint8_write(const miseg_checkpoint8_desc*, hipStream_t);
+int launch_checkpoint8_read(const miseg_checkpoint8_desc*, hipStream_t);
+long long group_norm_workspace(int, long long, int, int);
 int launch_image_minmax(const void*, int, int, long long, float*, hipStream_t);
 int launch_image_normalize(const void*, int, int, long long, const float*, float*, hipStream_t);
 int launch_resize_bilinear(const void*, int, float*, int, int, int, int, int, int, hipStream_t);
@@ -364,6 +369,25 @@ int miseg_bn_relu_bwd_apply(const void* x, const void* dy, void* dx, int64_t pix
 int miseg_bn_bwd_sums(const double* stats, int32_t replicas, int32_t stride, int32_t C, const float* mean,
                       const float* var, float eps, double* sums, void* stream) {
   return launch_bn_bwd_sums(stats, replicas, stride, C, mean, var, eps, sums, (hipStream_t)stream);
+}
+int64_t miseg_group_norm_workspace(int32_t N, int64_t pixels, int32_t C, int32_t backward) {
+  return group_norm_workspace(N, pixels, C, backward);
+}
+int miseg_group_norm_act_fwd(const miseg_group_norm_desc* d, void* stream) {
+  MISEG_CHECK_ARG(d, "group_norm_act: null descriptor");
+  return launch_group_norm_fwd(d, (hipStream_t)stream);
+}
+int miseg_group_norm_act_bwd(const miseg_group_norm_bwd_desc* d, void* stream) {
+  MISEG_CHECK_ARG(d, "group_norm_act_bwd: null descriptor");
+  return launch_group_norm_bwd(d, (hipStream_t)stream);
+}
+int miseg_checkpoint8_write(const miseg_checkpoint8_desc* d, void* stream) {
+  MISEG_CHECK_ARG(d, "checkpoint8_write: null descriptor");
+  return launch_checkpoint8_write(d, (hipStream_t)stream);
+}
+int miseg_checkpoint8_read(const miseg_checkpoint8_desc* d, void* stream) {
+  MISEG_CHECK_ARG(d, "checkpoint8_read: null descriptor");
+  return launch_checkpoint8_read(d, (hipStream_t)stream);
 }
 int miseg_image_minmax(const void* img, int32_t dtype, int32_t N, int64_t elems, float* minmax,
                        void* stream) {

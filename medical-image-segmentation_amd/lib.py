@@ -14,7 +14,7 @@ OK = 0
 E_INVALID_ARG, E_UNSUPPORTED_SHAPE, E_HIP, E_NO_DEVICE = -1, -2, -3, -4
 DT_BF16, DT_F32 = 0, 1
 FMT_BF16, FMT_F16 = 0, 1      # 16-bit storage format of activations and weights (miseg_conv_desc.fmt)
-ACT_NONE, ACT_RELU, ACT_SOFTMAX, ACT_SIGMOID = 0, 1, 2, 3
+ACT_NONE, ACT_RELU, ACT_SOFTMAX, ACT_SIGMOID, ACT_SILU = 0, 1, 2, 3, 4
 LOSS_CCE, LOSS_DICE, LOSS_FOCAL = 1, 2, 4
 RES_ADD, RES_BN_RELU_MASK = 0, 1
 TILE_NO_PERSIST = 128          # miseg_conv_desc.tile_hint flag: keep a layer off its persistent kernel
@@ -107,6 +107,42 @@ class WgradDesc(C.Structure):
     ]
 
 
+class GroupNormDesc(C.Structure):
+    """Mirror of `miseg_group_norm_desc`."""
+    _fields_ = [
+        ("x", C.c_void_p), ("y", C.c_void_p), ("gamma", C.c_void_p), ("beta", C.c_void_p),
+        ("mean", C.c_void_p), ("rstd", C.c_void_p), ("scale", C.c_void_p), ("shift", C.c_void_p),
+        ("codes", C.c_void_p), ("code_scales", C.c_void_p), ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_int64), ("pixels", C.c_int64), ("x_img", C.c_int64), ("y_img", C.c_int64),
+        ("x_pix", C.c_int32), ("y_pix", C.c_int32), ("N", C.c_int32), ("C", C.c_int32), ("groups", C.c_int32),
+        ("dtype", C.c_int32), ("fmt", C.c_int32), ("act", C.c_int32), ("eps", C.c_float),
+    ]
+
+
+class GroupNormBwdDesc(C.Structure):
+    """Mirror of `miseg_group_norm_bwd_desc`."""
+    _fields_ = [
+        ("x", C.c_void_p), ("codes", C.c_void_p), ("code_scales", C.c_void_p), ("dy", C.c_void_p),
+        ("dx", C.c_void_p), ("mean", C.c_void_p), ("rstd", C.c_void_p), ("scale", C.c_void_p),
+        ("shift", C.c_void_p), ("gamma", C.c_void_p), ("beta", C.c_void_p), ("dgamma", C.c_void_p),
+        ("dbeta", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64), ("pixels", C.c_int64),
+        ("x_img", C.c_int64), ("dy_img", C.c_int64), ("dx_img", C.c_int64),
+        ("x_pix", C.c_int32), ("dy_pix", C.c_int32), ("dx_pix", C.c_int32), ("N", C.c_int32), ("C", C.c_int32),
+        ("groups", C.c_int32), ("dtype", C.c_int32), ("fmt", C.c_int32), ("act", C.c_int32),
+    ]
+
+
+class Checkpoint8Desc(C.Structure):
+    """Mirror of `miseg_checkpoint8_desc`."""
+    _fields_ = [
+        ("x", C.c_void_p), ("y", C.c_void_p), ("codes", C.c_void_p), ("code_scales", C.c_void_p),
+        ("code_a", C.c_void_p), ("code_b", C.c_void_p), ("y_a", C.c_void_p), ("y_b", C.c_void_p),
+        ("pixels", C.c_int64), ("x_img", C.c_int64), ("y_img", C.c_int64), ("coef_img", C.c_int64),
+        ("x_pix", C.c_int32), ("y_pix", C.c_int32), ("N", C.c_int32), ("C", C.c_int32),
+        ("dtype", C.c_int32), ("fmt", C.c_int32), ("act", C.c_int32),
+    ]
+
+
 # name -> (restype, argtypes); every symbol include/miseg.h declares
 _VP, _I32, _I64, _FP = C.c_void_p, C.c_int32, C.c_int64, C.c_void_p
 SIGNATURES = {
@@ -149,6 +185,11 @@ SIGNATURES = {
     "miseg_bn_bwd_sums": (C.c_int, [_VP, _I32, _I32, _I32, _FP, _FP, C.c_float, _VP, _VP]),
     "miseg_bn_relu_bwd_apply": (C.c_int, [_VP, _VP, _VP, _I64, _I32, _I32, _I32, _I32, _FP, _FP, _FP,
                                           _FP, C.c_float, _I32, _VP, _VP, _I32, _VP]),
+    "miseg_group_norm_workspace": (C.c_int64, [_I32, _I64, _I32, _I32]),
+    "miseg_group_norm_act_fwd": (C.c_int, [C.POINTER(GroupNormDesc), _VP]),
+    "miseg_group_norm_act_bwd": (C.c_int, [C.POINTER(GroupNormBwdDesc), _VP]),
+    "miseg_checkpoint8_write": (C.c_int, [C.POINTER(Checkpoint8Desc), _VP]),
+    "miseg_checkpoint8_read": (C.c_int, [C.POINTER(Checkpoint8Desc), _VP]),
     "miseg_maxpool3x3s2_bwd": (C.c_int, [_VP, _VP, _VP, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _VP, _I32, _VP]),
     "miseg_avgpool2x2_bwd": (C.c_int, [_VP, _VP, _I32, _I32, _I32, _I32, _I32, _I32, _VP]),
     "miseg_maxpool2x2_fwd": (C.c_int, [_VP, _VP, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _VP]),
