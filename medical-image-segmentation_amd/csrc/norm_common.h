@@ -15,15 +15,42 @@ template <> struct Vec8<f32s> { uint4 v, w; };
 template <typename T> struct Elem { static constexpr int bytes = 2; };
 template <> struct Elem<f32s> { static constexpr int bytes = 4; };
 
-template <typename T> __device__ __forceinline__ Vec8<T> load8(const char* p) {
+// NT: the line is not kept in the caches (nontemporal).  Of 157 MB read twice, a second pass that also writes 157 MB takes
+// 38 us when the first left them in the 256 MB memory-side cache, 56 us when they come from HBM.
+typedef __attribute__((ext_vector_type(4))) unsigned nt_u32x4;
+template <bool NT> __device__ __forceinline__ uint4 load16(const char* p) {
+  if constexpr (NT) {
+    const nt_u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const nt_u32x4*>(p));
+    return make_uint4(v.x, v.y, v.z, v.w);
+  }
+  return *reinterpret_cast<const uint4*>(p);
+}
+template <bool NT> __device__ __forceinline__ void store16(char* p, uint4 v) {
+  if constexpr (NT) {
+    const nt_u32x4 w = {v.x, v.y, v.z, v.w};
+    __builtin_nontemporal_store(w, reinterpret_cast<nt_u32x4*>(p));
+  } else {
+    *reinterpret_cast<uint4*>(p) = v;
+  }
+}
+template <typename T, bool NT = false> __device__ __forceinline__ Vec8<T> load8(const char* p) {
   Vec8<T> r;
-  r.v = *reinterpret_cast<const uint4*>(p);
-  if constexpr (Elem<T>::bytes == 4) r.w = *reinterpret_cast<const uint4*>(p + 16);
+  r.v = load16<NT>(p);
+  if constexpr (Elem<T>::bytes == 4) r.w = load16<NT>(p + 16);
   return r;
 }
-template <typename T> __device__ __forceinline__ void store8(char* p, const Vec8<T>& r) {
-  *reinterpret_cast<uint4*>(p) = r.v;
-  if constexpr (Elem<T>::bytes == 4) *reinterpret_cast<uint4*>(p + 16) = r.w;
+template <typename T, bool NT = false> __device__ __forceinline__ void store8(char* p, const Vec8<T>& r) {
+  store16<NT>(p, r.v);
+  if constexpr (Elem<T>::bytes == 4) store16<NT>(p + 16, r.w);
+}
+// 8 codes
+typedef __attribute__((ext_vector_type(2))) unsigned nt_u32x2;
+template <bool NT> __device__ __forceinline__ uint2 load_codes(const signed char* p) {
+  if constexpr (NT) {
+    const nt_u32x2 v = __builtin_nontemporal_load(reinterpret_cast<const nt_u32x2*>(p));
+    return make_uint2(v.x, v.y);
+  }
+  return *reinterpret_cast<const uint2*>(p);
 }
 
 typedef __attribute__((ext_vector_type(2))) _Float16 nf16x2;
@@ -87,17 +114,18 @@ struct NormGrid {
   int chunk, blocks;                               // pixels per block (a multiple of rows), blocks per image
 };
 
-// Blocks enough to fill the chip (`want` in all), but none with less than `least` sweeps.
+// Blocks enough to fill the chip (`want` in all), none with less than `least` sweeps unless there are few of them anyway.
 static inline NormGrid norm_grid(long long N, long long pixels, int C, int want, int least) {
   NormGrid g;
   const int c8 = ((C + 31) / 32) * 4;
   g.ny = (c8 + 63) / 64;
   g.cw = ((c8 + g.ny - 1) / g.ny + 3) / 4 * 4;
   g.rows = kNormThreads / g.cw;
+  const long long sweeps = (pixels + g.rows - 1) / g.rows, all = sweeps * N * g.ny;
+  if (all < (long long)least * 1024) least = (int)(all / 1024) + 1;
   long long b = (want + N * g.ny - 1) / (N * g.ny);
-  const long long most = (pixels + (long long)g.rows * least - 1) / ((long long)g.rows * least);
+  const long long most = (sweeps + least - 1) / least;
   if (b > most) b = most;
-  if (b < 1) b = 1;
   long long chunk = (pixels + b - 1) / b;
   chunk = (chunk + g.rows - 1) / g.rows * g.rows;
   g.chunk = (int)chunk;
@@ -106,14 +134,14 @@ static inline NormGrid norm_grid(long long N, long long pixels, int C, int want,
 }
 
 struct NormWalk {
-  long long p0, p1;                                // pixels of this block
+  int p0, p1;                                      // pixels of this block
   int c, r, n;                                     // first channel, pixel of the sweep, image
   bool active;
-  __device__ __forceinline__ NormWalk(const NormGrid& g, long long pixels, int C) {
+  __device__ __forceinline__ NormWalk(const NormGrid& g, int block, int pixels, int C) {
     r = threadIdx.x / g.cw;
     c = (blockIdx.y * g.cw + threadIdx.x - r * g.cw) * 8;
     n = blockIdx.z;
-    p0 = (long long)blockIdx.x * g.chunk;
+    p0 = block * g.chunk;
     p1 = p0 + g.chunk < pixels ? p0 + g.chunk : pixels;
     active = r < g.rows && c < C;
   }
@@ -130,7 +158,11 @@ __device__ __forceinline__ void load_coef(float (&f)[8], const float* p) {
 // half a step.  Below 2^-119 the scale would be a subnormal number and its reciprocal infinite: such a block is zero.  A
 // value that is not finite makes the scale NaN, so that all of its block reads back as NaN and an overflow is not lost.
 struct Quant8 { uint2 codes; bf16_t scale; };
+// The definition's operations are single 32-bit roundings: m / 127 and 1 / scale, here by a reciprocal and a correction
+// (equal to the rounded quotient for every magnitude that is kept and for every bf16 scale), v * (1 / scale), and rint, by
+// adding 1.5 * 2^23: the sum's lowest byte is the code.  No product may be contracted into a sum, except in corrections.
 __device__ __forceinline__ Quant8 quantise8(const float (&v)[8]) {
+#pragma clang fp contract(off)
   unsigned m = 0;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {                    // magnitudes compared as integers: a NaN is above infinity
@@ -144,15 +176,24 @@ __device__ __forceinline__ Quant8 quantise8(const float (&v)[8]) {
   }
   Quant8 q;
   const float amax = __uint_as_float(m);
-  float s = amax < 0x1p-119f ? 0.f : amax / 127.f;
-  q.scale = m >= 0x7f800000u ? (bf16_t)0x7fc0 : f32_to_bf16(s);
+  float s = amax * (1.f / 127.f);
+  s = fmaf(fmaf(-127.f, s, amax), 1.f / 127.f, s);
+  q.scale = m >= 0x7f800000u ? (bf16_t)0x7fc0 : amax < 0x1p-119f ? (bf16_t)0 : f32_to_bf16(s);
   s = bf16_to_f32(q.scale);
-  const float inv = s > 0.f ? 1.f / s : 0.f;       // 0 for a zero and for a NaN scale
-  unsigned w[2] = {0, 0};
+  float inv = __builtin_amdgcn_rcpf(s);
+  inv = fmaf(fmaf(-s, inv, 1.f), inv, inv);
+  unsigned w[2];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float f = inv > 0.f ? rintf(v[j] * inv) : 0.f;
-    w[j >> 2] |= ((unsigned)(int)f & 0xffu) << (8 * (j & 3));
+  for (int h = 0; h < 2; ++h) {
+    unsigned b[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float t = v[4 * h + j] * inv;
+      b[j] = __float_as_uint(t + 12582912.f);
+    }
+    w[h] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(b[3], b[2], 0x0c0c0400), __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400),
+                                 0x05040100);
+    if (!(s > 0.f)) w[h] = 0;                      // a zero or NaN scale
   }
   q.codes = make_uint2(w[0], w[1]);
   return q;

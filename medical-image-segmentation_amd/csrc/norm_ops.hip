@@ -9,29 +9,30 @@ namespace miseg {
 // first value, so that an offset of the channel that is large against its spread does not cancel; threads and blocks are
 // joined by counts, means and sums of squares.
 template <typename T>
-__global__ __launch_bounds__(kNormThreads) void gn_stats_kernel(const char* x, long long xps, long long ximg,
-                                                                long long pixels, int C, NormGrid g,
-                                                                float2* __restrict__ part) {
+__global__ __launch_bounds__(kNormThreads) void gn_stats_kernel(const char* x, long long xps, long long ximg, int pixels,
+                                                                int C, NormGrid g, float2* __restrict__ part) {
   constexpr int ES = Elem<T>::bytes, U = 4;
   __shared__ float lmean[kNormThreads * 8], lm2[kNormThreads * 8];
   __shared__ int lcount[kNormThreads];
-  NormWalk w(g, pixels, C);
+  __shared__ double2 lsum[kNormThreads];
+  NormWalk w(g, blockIdx.x, pixels, C);
   float k[8], s1[8], s2[8];
   int count = 0;
 #pragma unroll
   for (int j = 0; j < 8; ++j) k[j] = s1[j] = s2[j] = 0.f;
-  if (w.active && w.p0 + w.r < w.p1) {
-    const char* xp = x + (w.n * ximg + w.c) * ES;
-    long long p = w.p0 + w.r;
-    unpack8(k, load8<T>(xp + p * xps * ES));
-    for (; p < w.p1; p += U * g.rows) {
+  int px = w.p0 + w.r;
+  if (w.active && px < w.p1) {
+    const char* xp = x + (w.n * ximg + px * xps + w.c) * ES;
+    const long long step = g.rows * xps * ES;
+    unpack8(k, load8<T>(xp));
+    for (; px < w.p1; px += U * g.rows, xp += U * step) {
       Vec8<T> v[U];
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (p + u * g.rows < w.p1) v[u] = load8<T>(xp + (p + u * g.rows) * xps * ES);
+        if (px + u * g.rows < w.p1) v[u] = load8<T>(xp + u * step);
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (p + u * g.rows < w.p1) {
+        if (px + u * g.rows < w.p1) {
           float f[8];
           unpack8(f, v[u]);
 #pragma unroll
@@ -45,26 +46,38 @@ __global__ __launch_bounds__(kNormThreads) void gn_stats_kernel(const char* x, l
     }
   }
   const float rc = count ? 1.f / (float)count : 0.f;
-  const int l = threadIdx.x - w.r * g.cw;
-  if (l == 0) lcount[w.r] = count;
+  if ((int)threadIdx.x == w.r * g.cw) lcount[w.r] = count;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     lmean[threadIdx.x * 8 + j] = k[j] + s1[j] * rc;
     lm2[threadIdx.x * 8 + j] = s2[j] - s1[j] * s1[j] * rc;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < g.cw * 8; i += kNormThreads) {
-    const int c = blockIdx.y * g.cw * 8 + i;
-    if (c >= C) break;
-    double n = 0, sum = 0, q = 0;
-    for (int r = 0; r < g.rows; ++r) {
-      const double m = lmean[r * g.cw * 8 + i];
-      n += lcount[r];
-      sum += lcount[r] * m;
-      q += lm2[r * g.cw * 8 + i] + lcount[r] * m * m;
+  // channel i of the slab from `parts` threads, then from one
+  const int wide = g.cw * 8, parts = wide < kNormThreads ? kNormThreads / wide : 1;
+  for (int i0 = 0; i0 < wide; i0 += kNormThreads) {
+    const int i = i0 + (int)threadIdx.x % wide, q = (int)threadIdx.x / wide;
+    double sum = 0, sq = 0;
+    if (q < parts && i < wide)
+      for (int r = q; r < g.rows; r += parts) {
+        const double m = lmean[r * wide + i], n = lcount[r];
+        sum += n * m;
+        sq += lm2[r * wide + i] + n * m * m;
+      }
+    if (parts > 1) {
+      lsum[threadIdx.x] = make_double2(sum, sq);
+      __syncthreads();
+      if (q == 0)
+        for (int t = 1; t < parts; ++t) {
+          sum += lsum[t * wide + i].x;
+          sq += lsum[t * wide + i].y;
+        }
     }
-    const double mean = sum / n;
-    part[((long long)w.n * gridDim.x + blockIdx.x) * C + c] = make_float2((float)mean, (float)(q - sum * mean));
+    const int c = blockIdx.y * wide + i;
+    if (q == 0 && i < wide && c < C) {
+      const double mean = sum / (w.p1 - w.p0);
+      part[((long long)w.n * gridDim.x + blockIdx.x) * C + c] = make_float2((float)mean, (float)(sq - sum * mean));
+    }
   }
 }
 
@@ -89,14 +102,24 @@ __global__ __launch_bounds__(kNormThreads) void gn_finalize_kernel(const float2*
   __shared__ double lds[4];
   const int w = C / groups, g = blockIdx.x, n = blockIdx.y;
   double s = 0, q = 0;
-  const long long entries = (long long)blocks * w;
-  for (long long e = threadIdx.x; e < entries; e += kNormThreads) {
-    const int b = (int)(e / w), c = g * w + (int)(e - (long long)b * w);
-    const float2 v = part[((long long)n * blocks + b) * C + c];
-    const long long left = pixels - (long long)b * chunk;
-    const double count = (double)(left < chunk ? left : chunk), m = v.x;
-    s += count * m;
-    q += (double)v.y + count * m * m;
+  const int entries = blocks * w, last = (int)(pixels - (long long)(blocks - 1) * chunk);
+  const float2* pp = part + (long long)n * blocks * C + g * w;
+  constexpr int U = 8;                             // loads in flight: the kernel waits for nothing else
+  for (int e0 = threadIdx.x; e0 < entries; e0 += U * kNormThreads) {
+    float2 v[U];
+    int count[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int e = e0 + u * kNormThreads, b = e / w;
+      count[u] = e >= entries ? 0 : b == blocks - 1 ? last : chunk;
+      v[u] = e < entries ? pp[(long long)b * C + (e - b * w)] : make_float2(0.f, 0.f);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const double n = count[u], m = v[u].x;
+      s += n * m;
+      q += (double)v[u].y + n * m * m;
+    }
   }
   s = block_sum(s, lds);
   q = block_sum(q, lds);
@@ -122,58 +145,68 @@ __global__ __launch_bounds__(kNormThreads) void gn_finalize_kernel(const float2*
 
 // ---------------------------------------------------------------------------- one pass: activated result, checkpoint
 // y = act(x a + b) and the checkpoint of x s + t (of x without s), either or both.  Coefficients per channel, `cimg` from
-// one image's to the next's.
+// one image's to the next's.  A block makes one sweep of U pixels per thread where there is work for 32768 blocks: short
+// blocks keep more loads and stores in flight than long walks (operand of 4 x 960 x 1280 x 64 out of 8 bits: 200 us with
+// 4096 blocks, 158 with 32768).  x is read for the last time here and y is read by another kernel: neither stays in the
+// caches.  The last pixels come first, as they are the likeliest to be in the caches still.
 struct PassArgs {
   const char* x;
   char* y;
   signed char* codes;
   bf16_t* scales;
   const float *a, *b, *s, *t;
-  long long pixels, xps, ximg, yps, yimg, cimg;
-  int C;
+  long long xps, ximg, yps, yimg, cimg;
+  int pixels, C;
   NormGrid g;
 };
 
 template <typename T, int ACT, bool Y, bool Q>
 __global__ __launch_bounds__(kNormThreads) void norm_pass_kernel(PassArgs p) {
   constexpr int ES = Elem<T>::bytes, U = 4;
-  NormWalk w(p.g, p.pixels, p.C);
+  NormWalk w(p.g, gridDim.x - 1 - blockIdx.x, p.pixels, p.C);
   if (w.r >= p.g.rows) return;                    // lanes past the last channel stay for the exchange in quantise8
   float a[8], b[8], s[8], t[8];
   if (w.active) {
     if (Y) { load_coef(a, p.a + w.n * p.cimg + w.c); load_coef(b, p.b + w.n * p.cimg + w.c); }
     if (Q && p.s) { load_coef(s, p.s + w.n * p.cimg + w.c); load_coef(t, p.t + w.n * p.cimg + w.c); }
   }
-  const char* xp = p.x + (w.n * p.ximg + w.c) * ES;
-  char* yp = p.y + (w.n * p.yimg + w.c) * ES;
-  const int blocks32 = (p.C + 31) >> 5;
-  for (long long px = w.p0 + w.r; px < w.p1; px += U * p.g.rows) {
+  const int blocks32 = (p.C + 31) >> 5, rows = p.g.rows;
+  int px = w.p0 + w.r;
+  const char* xp = p.x + (w.n * p.ximg + px * p.xps + w.c) * ES;
+  char* yp = p.y + (w.n * p.yimg + px * p.yps + w.c) * ES;
+  const long long row = (long long)w.n * p.pixels + px, xstep = rows * p.xps * ES, ystep = rows * p.yps * ES;
+  signed char* cp = p.codes + row * p.C + w.c;
+  bf16_t* sp = p.scales + row * blocks32 + (w.c >> 5);
+  const int cstep = rows * p.C, sstep = rows * blocks32;
+  for (; px < w.p1; px += U * rows) {
     Vec8<T> v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (w.active && px + u * p.g.rows < w.p1) v[u] = load8<T>(xp + (px + u * p.g.rows) * p.xps * ES);
+      if (w.active && px + u * rows < w.p1) v[u] = load8<T, true>(xp + u * xstep);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const long long at = px + u * p.g.rows;
-      if (at >= w.p1) break;
+      if (px + u * rows >= w.p1) break;
       float f[8], o[8];
       if (w.active) unpack8(f, v[u]);
       if (Y && w.active) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) o[j] = act_fwd<ACT>(fmaf(f[j], a[j], b[j]));
-        store8<T>(yp + at * p.yps * ES, pack8<T>(o));
+        store8<T, true>(yp + u * ystep, pack8<T>(o));
       }
       if constexpr (Q) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) o[j] = !w.active ? 0.f : p.s ? fmaf(f[j], s[j], t[j]) : f[j];
         const Quant8 q = quantise8(o);
-        const long long row = w.n * p.pixels + at;
         if (w.active) {
-          *reinterpret_cast<uint2*>(p.codes + row * p.C + w.c) = q.codes;
-          if ((w.c & 31) == 0) p.scales[row * blocks32 + (w.c >> 5)] = q.scale;
+          *reinterpret_cast<uint2*>(cp + u * cstep) = q.codes;
+          if ((w.c & 31) == 0) sp[u * sstep] = q.scale;
         }
       }
     }
+    xp += U * xstep;
+    yp += U * ystep;
+    cp += U * cstep;
+    sp += U * sstep;
   }
 }
 
@@ -184,40 +217,46 @@ struct ReadArgs {
   const bf16_t* scales;
   char* y;
   const float *a, *b;
-  long long pixels, yps, yimg, cimg;
-  int C;
+  long long yps, yimg, cimg;
+  int pixels, C;
   NormGrid g;
 };
 
 template <typename T, int ACT, bool AFF>
 __global__ __launch_bounds__(kNormThreads) void checkpoint_read_kernel(ReadArgs p) {
   constexpr int ES = Elem<T>::bytes, U = 4;
-  NormWalk w(p.g, p.pixels, p.C);
+  NormWalk w(p.g, blockIdx.x, p.pixels, p.C);
   if (!w.active) return;
   float a[8], b[8];
   if (AFF) { load_coef(a, p.a + w.n * p.cimg + w.c); load_coef(b, p.b + w.n * p.cimg + w.c); }
-  const int blocks32 = (p.C + 31) >> 5;
-  const signed char* cp = p.codes + w.n * p.pixels * p.C + w.c;
-  const bf16_t* sp = p.scales + w.n * p.pixels * blocks32 + (w.c >> 5);
-  char* yp = p.y + (w.n * p.yimg + w.c) * ES;
-  for (long long px = w.p0 + w.r; px < w.p1; px += U * p.g.rows) {
+  const int blocks32 = (p.C + 31) >> 5, rows = p.g.rows;
+  int px = w.p0 + w.r;
+  const long long row = (long long)w.n * p.pixels + px, ystep = rows * p.yps * ES;
+  const signed char* cp = p.codes + row * p.C + w.c;
+  const bf16_t* sp = p.scales + row * blocks32 + (w.c >> 5);
+  char* yp = p.y + (w.n * p.yimg + px * p.yps + w.c) * ES;
+  const int cstep = rows * p.C, sstep = rows * blocks32;
+  for (; px < w.p1; px += U * rows) {
     uint2 q[U];
     bf16_t s[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (px + u * p.g.rows < w.p1) {
-        q[u] = *reinterpret_cast<const uint2*>(cp + (px + u * p.g.rows) * p.C);
-        s[u] = sp[(px + u * p.g.rows) * blocks32];
+      if (px + u * rows < w.p1) {
+        q[u] = load_codes<true>(cp + u * cstep);
+        s[u] = sp[u * sstep];
       }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (px + u * p.g.rows >= w.p1) break;
+      if (px + u * rows >= w.p1) break;
       float f[8];
       dequantise8(f, q[u], bf16_to_f32(s[u]));
 #pragma unroll
       for (int j = 0; j < 8; ++j) f[j] = act_fwd<ACT>(AFF ? fmaf(f[j], a[j], b[j]) : f[j]);
-      store8<T>(yp + (px + u * p.g.rows) * p.yps * ES, pack8<T>(f));
+      store8<T, true>(yp + u * ystep, pack8<T>(f));
     }
+    cp += U * cstep;
+    sp += U * sstep;
+    yp += U * ystep;
   }
 }
 
@@ -231,8 +270,10 @@ struct BwdArgs {
   const bf16_t* scales;
   const float *mean, *rstd, *a, *b, *gamma, *beta; // mean, rstd [N][groups]; a, b [N][C]; gamma, beta [C] (checkpoint)
   const float *cm, *cp, *cq;                       // [N][C], second pass: dx = a g + (x - cm) cp + cq
-  long long pixels, xps, ximg, dps, dimg, ops, oimg;
-  int C, groups;
+  const double2* sums;                             // [N][C], all images: second pass, where the parameters' gradients are due
+  float *dgamma, *dbeta;
+  long long xps, ximg, dps, dimg, ops, oimg;
+  int pixels, C, groups, images;
   NormGrid g;
 };
 
@@ -245,18 +286,49 @@ template <typename T> struct BwdLoad<T, true> {
   Vec8<T> dy;
 };
 
-template <typename T, bool CK>
-__device__ __forceinline__ void bwd_load(BwdLoad<T, CK>& l, const BwdArgs& p, const NormWalk& w, long long at, int blocks32) {
-  constexpr int ES = Elem<T>::bytes;
-  if constexpr (CK) {
-    const long long row = w.n * p.pixels + at;
-    l.codes = *reinterpret_cast<const uint2*>(p.codes + row * p.C + w.c);
-    l.scale = p.scales[row * blocks32 + (w.c >> 5)];
-  } else {
-    l.x = load8<T>(p.x + (w.n * p.ximg + at * p.xps + w.c) * ES);
+// Where a thread's next pixels lie.
+template <typename T, bool CK> struct BwdFrom {
+  const char *x, *dy;
+  const signed char* codes;
+  const bf16_t* scales;
+  long long xstep, dstep;
+  int cstep, sstep;
+  __device__ __forceinline__ BwdFrom(const BwdArgs& p, const NormWalk& w) {
+    constexpr int ES = Elem<T>::bytes;
+    const int px = w.p0 + w.r, blocks32 = (p.C + 31) >> 5;
+    if constexpr (CK) {
+      const long long row = (long long)w.n * p.pixels + px;
+      codes = p.codes + row * p.C + w.c;
+      scales = p.scales + row * blocks32 + (w.c >> 5);
+      cstep = p.g.rows * p.C;
+      sstep = p.g.rows * blocks32;
+    } else {
+      x = p.x + (w.n * p.ximg + px * p.xps + w.c) * ES;
+      xstep = p.g.rows * p.xps * ES;
+    }
+    dy = p.dy + (w.n * p.dimg + px * p.dps + w.c) * ES;
+    dstep = p.g.rows * p.dps * ES;
   }
-  l.dy = load8<T>(p.dy + (w.n * p.dimg + at * p.dps + w.c) * ES);
-}
+  // XNT, DNT: keep x (the codes), dy out of the caches
+  template <bool XNT, bool DNT> __device__ __forceinline__ void load(BwdLoad<T, CK>& l, int u) const {
+    if constexpr (CK) {
+      l.codes = load_codes<XNT>(codes + u * cstep);
+      l.scale = scales[u * sstep];
+    } else {
+      l.x = load8<T, XNT>(x + u * xstep);
+    }
+    l.dy = load8<T, DNT>(dy + u * dstep);
+  }
+  __device__ __forceinline__ void next(int u) {
+    if constexpr (CK) {
+      codes += u * cstep;
+      scales += u * sstep;
+    } else {
+      x += u * xstep;
+    }
+    dy += u * dstep;
+  }
+};
 
 // Coefficients of z for this thread's channels.
 template <bool CK>
@@ -273,12 +345,14 @@ __device__ __forceinline__ void bwd_coef(float (&za)[8], float (&zb)[8], const B
   }
 }
 
-// First pass: per block and channel sum g and sum g xhat.
-template <typename T, int ACT, bool CK>
+// First pass: per block and channel sum g and sum g xhat.  XNT: x does not stay in the caches, as it and dy together are more
+// than they hold.
+template <typename T, int ACT, bool CK, bool XNT>
 __global__ __launch_bounds__(kNormThreads) void gn_bwd_reduce_kernel(BwdArgs p, float2* __restrict__ part) {
   constexpr int U = 4;
   __shared__ float l1[kNormThreads * 8], l2[kNormThreads * 8];
-  NormWalk w(p.g, p.pixels, p.C);
+  __shared__ double2 lsum[kNormThreads];
+  NormWalk w(p.g, blockIdx.x, p.pixels, p.C);
   float s1[8], s2[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) s1[j] = s2[j] = 0.f;
@@ -294,15 +368,16 @@ __global__ __launch_bounds__(kNormThreads) void gn_bwd_reduce_kernel(BwdArgs p, 
         rs[j] = p.rstd[at];
       }
     }
-    const int blocks32 = (p.C + 31) >> 5;
-    for (long long px = w.p0 + w.r; px < w.p1; px += U * p.g.rows) {
+    BwdFrom<T, CK> from(p, w);
+    const int rows = p.g.rows;
+    for (int px = w.p0 + w.r; px < w.p1; px += U * rows, from.next(U)) {
       BwdLoad<T, CK> l[U];
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (px + u * p.g.rows < w.p1) bwd_load<T, CK>(l[u], p, w, px + u * p.g.rows, blocks32);
+        if (px + u * rows < w.p1) from.template load<XNT, false>(l[u], u);
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (px + u * p.g.rows < w.p1) {
+        if (px + u * rows < w.p1) {
           float f[8], d[8];
           unpack8(d, l[u].dy);
           if constexpr (CK) dequantise8(f, l[u].codes, bf16_to_f32(l[u].scale));
@@ -326,15 +401,27 @@ __global__ __launch_bounds__(kNormThreads) void gn_bwd_reduce_kernel(BwdArgs p, 
     l2[threadIdx.x * 8 + j] = s2[j];
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < p.g.cw * 8; i += kNormThreads) {
-    const int c = blockIdx.y * p.g.cw * 8 + i;
-    if (c >= p.C) break;
+  const int wide = p.g.cw * 8, parts = wide < kNormThreads ? kNormThreads / wide : 1;
+  for (int i0 = 0; i0 < wide; i0 += kNormThreads) {
+    const int i = i0 + (int)threadIdx.x % wide, q = (int)threadIdx.x / wide;
     double a = 0, b = 0;
-    for (int r = 0; r < p.g.rows; ++r) {
-      a += l1[r * p.g.cw * 8 + i];
-      b += l2[r * p.g.cw * 8 + i];
+    if (q < parts && i < wide)
+      for (int r = q; r < p.g.rows; r += parts) {
+        a += l1[r * wide + i];
+        b += l2[r * wide + i];
+      }
+    if (parts > 1) {
+      lsum[threadIdx.x] = make_double2(a, b);
+      __syncthreads();
+      if (q == 0)
+        for (int t = 1; t < parts; ++t) {
+          a += lsum[t * wide + i].x;
+          b += lsum[t * wide + i].y;
+        }
     }
-    part[((long long)w.n * gridDim.x + blockIdx.x) * p.C + c] = make_float2((float)a, (float)b);
+    const int c = blockIdx.y * wide + i;
+    if (q == 0 && i < wide && c < p.C)
+      part[((long long)w.n * gridDim.x + blockIdx.x) * p.C + c] = make_float2((float)a, (float)b);
   }
 }
 
@@ -351,6 +438,7 @@ __global__ __launch_bounds__(kNormThreads) void gn_bwd_finalize_kernel(BwdArgs p
     const int c = g * w + c0 + ci;
     double a = 0, b = 0;
     if (li < lanes && c0 + ci < w)
+#pragma unroll 8
       for (int k = li; k < blocks; k += lanes) {
         const float2 v = part[((long long)n * blocks + k) * p.C + c];
         a += v.x;
@@ -388,12 +476,11 @@ __global__ __launch_bounds__(kNormThreads) void gn_bwd_finalize_kernel(BwdArgs p
   }
 }
 
-__global__ __launch_bounds__(kNormThreads) void gn_bwd_params_kernel(const double2* __restrict__ sums, int N, int C,
-                                                                     float* __restrict__ dgamma, float* __restrict__ dbeta) {
-  const int c = blockIdx.x * kNormThreads + threadIdx.x;
-  if (c >= C) return;
+// The parameters' gradients: the images' sums.
+__device__ __forceinline__ void gn_bwd_params(const double2* sums, int images, int C, int c, float* dgamma, float* dbeta) {
   double a = 0, b = 0;
-  for (int n = 0; n < N; ++n) {
+#pragma unroll 8
+  for (int n = 0; n < images; ++n) {
     const double2 v = sums[(long long)n * C + c];
     a += v.x;
     b += v.y;
@@ -402,11 +489,17 @@ __global__ __launch_bounds__(kNormThreads) void gn_bwd_params_kernel(const doubl
   if (dgamma) dgamma[c] = (float)b;
 }
 
-// Second pass: dx = a g + (x - cm) cp + cq.
+// Second pass: dx = a g + (x - cm) cp + cq.  With `sums`, the blocks past the last pixels add up the parameters' gradients.
 template <typename T, int ACT, bool CK>
 __global__ __launch_bounds__(kNormThreads) void gn_bwd_apply_kernel(BwdArgs p) {
   constexpr int ES = Elem<T>::bytes, U = 4;
-  NormWalk w(p.g, p.pixels, p.C);
+  if ((int)blockIdx.x == p.g.blocks) {
+    if (blockIdx.z == 0)
+      for (int i = threadIdx.x; i < p.g.cw * 8; i += kNormThreads)
+        if (const int c = blockIdx.y * p.g.cw * 8 + i; c < p.C) gn_bwd_params(p.sums, p.images, p.C, c, p.dgamma, p.dbeta);
+    return;
+  }
+  NormWalk w(p.g, p.g.blocks - 1 - blockIdx.x, p.pixels, p.C);
   if (!w.active) return;
   float za[8], zb[8], a[8], m[8], kp[8], kq[8];
   const long long cat = (long long)w.n * p.C + w.c;
@@ -415,16 +508,19 @@ __global__ __launch_bounds__(kNormThreads) void gn_bwd_apply_kernel(BwdArgs p) {
   load_coef(kp, p.cp + cat);
   load_coef(kq, p.cq + cat);
   if constexpr (!CK) load_coef(m, p.cm + cat);
-  const int blocks32 = (p.C + 31) >> 5;
-  for (long long px = w.p0 + w.r; px < w.p1; px += U * p.g.rows) {
+  BwdFrom<T, CK> from(p, w);
+  const int rows = p.g.rows;
+  int px = w.p0 + w.r;
+  char* op = p.dx + (w.n * p.oimg + px * p.ops + w.c) * ES;
+  const long long ostep = rows * p.ops * ES;
+  for (; px < w.p1; px += U * rows, from.next(U), op += U * ostep) {
     BwdLoad<T, CK> l[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (px + u * p.g.rows < w.p1) bwd_load<T, CK>(l[u], p, w, px + u * p.g.rows, blocks32);
+      if (px + u * rows < w.p1) from.template load<true, true>(l[u], u);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const long long at = px + u * p.g.rows;
-      if (at >= w.p1) break;
+      if (px + u * rows >= w.p1) break;
       float f[8], d[8];
       unpack8(d, l[u].dy);
       if constexpr (CK) dequantise8(f, l[u].codes, bf16_to_f32(l[u].scale));
@@ -434,7 +530,7 @@ __global__ __launch_bounds__(kNormThreads) void gn_bwd_apply_kernel(BwdArgs p) {
         const float gj = act_bwd<ACT>(fmaf(f[j], za[j], zb[j]), d[j]);
         d[j] = fmaf(a[j], gj, fmaf(CK ? f[j] : f[j] - m[j], kp[j], kq[j]));
       }
-      store8<T>(p.dx + (w.n * p.oimg + at * p.ops + w.c) * ES, pack8<T>(d));
+      store8<T, true>(op + u * ostep, pack8<T>(d));
     }
   }
 }
@@ -474,14 +570,30 @@ static bool good_view(const void* p, int pix, long long img, long long N, long l
 static bool good_coef(const void* p) { return ((uintptr_t)p & 15) == 0; }
 static int bytes_of(int dtype) { return dtype == MISEG_DT_F32 ? 4 : 2; }
 
-constexpr int kStatBlocks = 2048, kStatLeast = 8;  // blocks of a reduction, sweeps in the smallest of them
-constexpr int kPassBlocks = 4096, kPassLeast = 4;  // the same for a pass that only streams
+constexpr int kStatBlocks = 512, kStatLeast = 8;   // blocks of a reduction, sweeps in the smallest of them
+constexpr int kPassBlocks = 32768, kPassLeast = 4; // the same for a pass that only streams
+// Images are taken one launch after the other in steps whose tensors stay in the memory-side cache (256 MB) from the first
+// pass to the second.
+constexpr long long kCacheBytes = 200000000;
+
+static int images_per_step(long long N, long long image_bytes) {
+  const long long n = kCacheBytes / image_bytes;
+  return (int)(n < 1 ? 1 : n < N ? n : N);
+}
 
 static long long round_up(long long v) { return (v + 255) / 256 * 256; }
 
+// The blocks' partial sums, for steps of any number of images: norm_grid gives at most max(want, images x slabs) + images x
+// slabs - 1 blocks over all slabs, and a block writes cw * 8 channels at most.
+static long long gn_partials(long long N, long long pixels, int C) {
+  const NormGrid g = norm_grid(1, pixels, C, kStatBlocks, 1);
+  const long long slab = 8LL * g.cw * 8, most = (long long)((pixels + g.rows - 1) / g.rows) * N * g.ny;
+  const long long blocks = kStatBlocks + 2 * N * g.ny;
+  return round_up(slab * (blocks < most ? blocks : most));
+}
+
 static long long gn_workspace(long long N, long long pixels, int C, int backward) {
-  const NormGrid g = norm_grid(N, pixels, C, kStatBlocks, kStatLeast);
-  const long long part = round_up(8LL * N * g.blocks * C), coef = round_up(4LL * N * C);
+  const long long part = gn_partials(N, pixels, C), coef = round_up(4LL * N * C);
   return backward ? part + 2 * round_up(8LL * N * C) + 3 * coef : part + 2 * coef;
 }
 
@@ -516,26 +628,36 @@ int launch_group_norm_fwd(const miseg_group_norm_desc* d, hipStream_t s) {
                   "group_norm_act: the workspace must be 16-byte aligned and hold %lld bytes (%lld given)", need,
                   (long long)d->workspace_bytes);
   const int storage = storage_of(d->dtype, d->fmt);
-  const NormGrid g = norm_grid(d->N, d->pixels, d->C, kStatBlocks, kStatLeast);
   char* ws = (char*)d->workspace;
   float2* part = (float2*)ws;
-  ws += round_up(8LL * d->N * g.blocks * d->C);
+  ws += gn_partials(d->N, d->pixels, d->C);
   float *qs = nullptr, *qt = nullptr;
   if (d->codes) {
     qs = (float*)ws;
     qt = (float*)(ws + round_up(4LL * d->N * d->C));
   }
-  const dim3 grid(g.blocks, g.ny, d->N);
-  by_type_act(storage, NA_NONE, [&](auto t, auto) {
-    hipLaunchKernelGGL((gn_stats_kernel<decltype(t)>), grid, dim3(kNormThreads), 0, s, (const char*)d->x, (long long)d->x_pix,
-                       d->x_img, d->pixels, d->C, g, part);
-  });
-  hipLaunchKernelGGL(gn_finalize_kernel, dim3(d->groups, d->N), dim3(kNormThreads), 0, s, part, g.blocks, g.chunk, d->pixels,
-                     d->C, d->groups, d->gamma, d->beta, d->eps, d->mean, d->rstd, d->scale, d->shift, qs, qt);
-  PassArgs p{(const char*)d->x, (char*)d->y, (signed char*)d->codes, (bf16_t*)d->code_scales, d->scale, d->shift, qs, qt,
-             d->pixels, d->x_pix, d->x_img, d->y_pix, d->y_img, d->C, d->C,
-             norm_grid(d->N, d->pixels, d->C, kPassBlocks, kPassLeast)};
-  launch_pass(p, d->N, storage, act_of(d->act), s);
+  const int step = images_per_step(d->N, d->pixels * d->C * bytes);
+  for (int n0 = 0; n0 < d->N; n0 += step) {
+    const int n = d->N - n0 < step ? d->N - n0 : step;
+    const char* x = (const char*)d->x + n0 * d->x_img * bytes;
+    const long long cat = (long long)n0 * d->C, gat = (long long)n0 * d->groups;
+    const NormGrid g = norm_grid(n, d->pixels, d->C, kStatBlocks, kStatLeast);
+    by_type_act(storage, NA_NONE, [&](auto t, auto) {
+      hipLaunchKernelGGL((gn_stats_kernel<decltype(t)>), dim3(g.blocks, g.ny, n), dim3(kNormThreads), 0, s, x,
+                         (long long)d->x_pix, d->x_img, (int)d->pixels, d->C, g, part);
+    });
+    hipLaunchKernelGGL(gn_finalize_kernel, dim3(d->groups, n), dim3(kNormThreads), 0, s, part, g.blocks, g.chunk, d->pixels,
+                       d->C, d->groups, d->gamma, d->beta, d->eps, d->mean + gat, d->rstd + gat, d->scale + cat,
+                       d->shift + cat, qs, qt);
+    PassArgs p{x, (char*)d->y + n0 * d->y_img * bytes, (signed char*)d->codes, (bf16_t*)d->code_scales, d->scale + cat,
+               d->shift + cat, qs, qt, d->x_pix, d->x_img, d->y_pix, d->y_img, d->C, (int)d->pixels, d->C,
+               norm_grid(n, d->pixels, d->C, kPassBlocks, kPassLeast)};
+    if (p.codes) {
+      p.codes += n0 * d->pixels * d->C;
+      p.scales += n0 * d->pixels * ((d->C + 31) / 32);
+    }
+    launch_pass(p, n, storage, act_of(d->act), s);
+  }
   MISEG_CHECK_HIP(hipGetLastError());
   return MISEG_OK;
 }
@@ -564,36 +686,51 @@ int launch_group_norm_bwd(const miseg_group_norm_bwd_desc* d, hipStream_t s) {
   const int storage = storage_of(d->dtype, d->fmt), act = act_of(d->act);
   const bool ck = d->codes != nullptr;
   char* ws = (char*)d->workspace;
-  const NormGrid g = norm_grid(d->N, d->pixels, d->C, kStatBlocks, kStatLeast);
   float2* part = (float2*)ws;
-  ws += round_up(8LL * d->N * g.blocks * d->C);
+  ws += gn_partials(d->N, d->pixels, d->C);
   double2* sums = (double2*)ws;
   ws += 2 * round_up(8LL * d->N * d->C);
   const long long coef = round_up(4LL * d->N * d->C);
   float *cm = (float*)ws, *cp = (float*)(ws + coef), *cq = (float*)(ws + 2 * coef);
-  BwdArgs p{(const char*)d->x, (const char*)d->dy, (char*)d->dx, (const signed char*)d->codes, (const bf16_t*)d->code_scales,
-            d->mean, d->rstd, d->scale, d->shift, d->gamma, d->beta, cm, cp, cq, d->pixels, d->x_pix, d->x_img, d->dy_pix,
-            d->dy_img, d->dx_pix, d->dx_img, d->C, d->groups, g};
-  by_type_act(storage, act, [&](auto t, auto a) {
-    typedef decltype(t) T;
-    constexpr int A = decltype(a)::act;
-    const dim3 grid(g.blocks, g.ny, d->N);
-    if (ck) hipLaunchKernelGGL((gn_bwd_reduce_kernel<T, A, true>), grid, dim3(kNormThreads), 0, s, p, part);
-    else hipLaunchKernelGGL((gn_bwd_reduce_kernel<T, A, false>), grid, dim3(kNormThreads), 0, s, p, part);
-  });
-  hipLaunchKernelGGL(gn_bwd_finalize_kernel, dim3(d->groups, d->N), dim3(kNormThreads), 0, s, p, part, g.blocks, ck ? 1 : 0,
-                     sums, cm, cp, cq);
-  if (d->dgamma || d->dbeta)
-    hipLaunchKernelGGL(gn_bwd_params_kernel, dim3((d->C + kNormThreads - 1) / kNormThreads), dim3(kNormThreads), 0, s, sums,
-                       d->N, d->C, d->dgamma, d->dbeta);
-  p.g = norm_grid(d->N, d->pixels, d->C, kPassBlocks, kPassLeast);
-  by_type_act(storage, act, [&](auto t, auto a) {
-    typedef decltype(t) T;
-    constexpr int A = decltype(a)::act;
-    const dim3 grid(p.g.blocks, p.g.ny, d->N);
-    if (ck) hipLaunchKernelGGL((gn_bwd_apply_kernel<T, A, true>), grid, dim3(kNormThreads), 0, s, p);
-    else hipLaunchKernelGGL((gn_bwd_apply_kernel<T, A, false>), grid, dim3(kNormThreads), 0, s, p);
-  });
+  const long long dbytes = d->pixels * d->C * bytes, xbytes = ck ? d->pixels * (d->C + 2 * ((d->C + 31) / 32)) : dbytes;
+  // both stay in the cache if they can; else dy alone; else the last pixels of both
+  const bool alone = xbytes + dbytes > kCacheBytes && dbytes <= kCacheBytes;
+  const int step = images_per_step(d->N, alone ? dbytes : xbytes + dbytes);
+  for (int n0 = 0; n0 < d->N; n0 += step) {
+    const int n = d->N - n0 < step ? d->N - n0 : step;
+    const long long cat = (long long)n0 * d->C, gat = (long long)n0 * d->groups;
+    BwdArgs p{(const char*)d->x + n0 * d->x_img * bytes, (const char*)d->dy + n0 * d->dy_img * bytes,
+              (char*)d->dx + n0 * d->dx_img * bytes, (const signed char*)d->codes, (const bf16_t*)d->code_scales,
+              d->mean + gat, d->rstd + gat, d->scale + cat, d->shift + cat, d->gamma, d->beta, cm, cp, cq, nullptr,
+              d->dgamma, d->dbeta, d->x_pix, d->x_img, d->dy_pix, d->dy_img, d->dx_pix, d->dx_img, (int)d->pixels, d->C,
+              d->groups, d->N, norm_grid(n, d->pixels, d->C, kStatBlocks, kStatLeast)};
+    if (ck) {
+      p.codes += n0 * d->pixels * d->C;
+      p.scales += n0 * d->pixels * ((d->C + 31) / 32);
+    }
+    const int blocks = p.g.blocks;
+    by_type_act(storage, act, [&](auto t, auto a) {
+      typedef decltype(t) T;
+      constexpr int A = decltype(a)::act;
+      const dim3 grid(blocks, p.g.ny, n);
+      if (ck && alone) hipLaunchKernelGGL((gn_bwd_reduce_kernel<T, A, true, true>), grid, dim3(kNormThreads), 0, s, p, part);
+      else if (ck) hipLaunchKernelGGL((gn_bwd_reduce_kernel<T, A, true, false>), grid, dim3(kNormThreads), 0, s, p, part);
+      else if (alone) hipLaunchKernelGGL((gn_bwd_reduce_kernel<T, A, false, true>), grid, dim3(kNormThreads), 0, s, p, part);
+      else hipLaunchKernelGGL((gn_bwd_reduce_kernel<T, A, false, false>), grid, dim3(kNormThreads), 0, s, p, part);
+    });
+    hipLaunchKernelGGL(gn_bwd_finalize_kernel, dim3(d->groups, n), dim3(kNormThreads), 0, s, p, part, blocks, ck ? 1 : 0,
+                       sums + cat, cm, cp, cq);
+    p.g = norm_grid(n, d->pixels, d->C, kPassBlocks, kPassLeast);
+    const bool params = n0 + n == d->N && (d->dgamma || d->dbeta);
+    if (params) p.sums = sums;
+    by_type_act(storage, act, [&](auto t, auto a) {
+      typedef decltype(t) T;
+      constexpr int A = decltype(a)::act;
+      const dim3 grid(p.g.blocks + (params ? 1 : 0), p.g.ny, n);
+      if (ck) hipLaunchKernelGGL((gn_bwd_apply_kernel<T, A, true>), grid, dim3(kNormThreads), 0, s, p);
+      else hipLaunchKernelGGL((gn_bwd_apply_kernel<T, A, false>), grid, dim3(kNormThreads), 0, s, p);
+    });
+  }
   MISEG_CHECK_HIP(hipGetLastError());
   return MISEG_OK;
 }
@@ -614,7 +751,7 @@ int launch_checkpoint8_write(const miseg_checkpoint8_desc* d, hipStream_t s) {
                             !views_clash(d->x, d->x_pix, d->x_img, d->y, d->y_pix, d->y_img, d->N, d->pixels, d->C, bytes)),
                   "checkpoint8_write: y must be a view like x, and be x, another channel range of its buffer or apart from it");
   PassArgs p{(const char*)d->x, (char*)d->y, (signed char*)d->codes, (bf16_t*)d->code_scales, d->y_a, d->y_b, d->code_a,
-             d->code_b, d->pixels, d->x_pix, d->x_img, d->y_pix, d->y_img, d->coef_img, d->C,
+             d->code_b, d->x_pix, d->x_img, d->y_pix, d->y_img, d->coef_img, (int)d->pixels, d->C,
              norm_grid(d->N, d->pixels, d->C, kPassBlocks, kPassLeast)};
   launch_pass(p, d->N, storage_of(d->dtype, d->fmt), act_of(d->act), s);
   MISEG_CHECK_HIP(hipGetLastError());
@@ -630,8 +767,8 @@ int launch_checkpoint8_read(const miseg_checkpoint8_desc* d, hipStream_t s) {
                   "checkpoint8_read: codes and code_scales are needed, 8-byte and 2-byte aligned");
   MISEG_CHECK_ARG(!d->y_a == !d->y_b && good_coef(d->y_a) && good_coef(d->y_b) && (d->coef_img & 3) == 0 && d->coef_img >= 0,
                   "checkpoint8_read: coefficients go in pairs, 16-byte aligned");
-  ReadArgs p{(const signed char*)d->codes, (const bf16_t*)d->code_scales, (char*)d->y, d->y_a, d->y_b, d->pixels, d->y_pix,
-             d->y_img, d->coef_img, d->C, norm_grid(d->N, d->pixels, d->C, kPassBlocks, kPassLeast)};
+  ReadArgs p{(const signed char*)d->codes, (const bf16_t*)d->code_scales, (char*)d->y, d->y_a, d->y_b, d->y_pix,
+             d->y_img, d->coef_img, (int)d->pixels, d->C, norm_grid(d->N, d->pixels, d->C, kPassBlocks, kPassLeast)};
   const dim3 grid(p.g.blocks, p.g.ny, d->N);
   by_type_act(storage_of(d->dtype, d->fmt), act_of(d->act), [&](auto t, auto a) {
     typedef decltype(t) T;
