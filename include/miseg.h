@@ -552,8 +552,8 @@ int miseg_bn_bwd_sums(const double* stats, int32_t replicas, int32_t stride, int
  * bytes, C of 8.  y may be x itself or another channel range of x's buffer and overlaps it in no other way.  Statistics
  * and sums are in fp32 per thread and fp64 across threads, without atomics: equal calls give equal bits.  Results are
  * rounded once; what exceeds the range of fp16 becomes an infinity.
- * workspace: miseg_group_norm_workspace(N, pixels, C, backward) bytes, 16-byte aligned, not cleared by anyone; calls that
- * overlap in time need one each.
+ * workspace: miseg_group_norm_workspace() bytes (none for the smallest maps), 16-byte aligned, not cleared by anyone; calls
+ * that overlap in time need one each.
  */
 typedef struct miseg_group_norm_desc {
   const void* x;
@@ -575,7 +575,8 @@ typedef struct miseg_group_norm_desc {
   int32_t dtype, fmt, act;
   float eps;
 } miseg_group_norm_desc;
-int64_t miseg_group_norm_workspace(int32_t N, int64_t pixels, int32_t C, int32_t backward);
+int64_t miseg_group_norm_workspace(int32_t N, int64_t pixels, int32_t C, int32_t groups, int32_t dtype, int32_t checkpoint,
+                                   int32_t backward);
 int miseg_group_norm_act_fwd(const miseg_group_norm_desc* d, void* stream);
 
 /*

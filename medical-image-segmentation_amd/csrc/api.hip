@@ -45,7 +45,7 @@ int launch_group_norm_fwd(const miseg_group_norm_desc*, hipStream_t);
 int launch_group_norm_bwd(const miseg_group_norm_bwd_desc*, hipStream_t);
 int launch_checkpoint8_write(const miseg_checkpoint8_desc*, hipStream_t);
 int launch_checkpoint8_read(const miseg_checkpoint8_desc*, hipStream_t);
-long long group_norm_workspace(int, long long, int, int);
+long long group_norm_workspace(int, long long, int, int, int, int, int);
 int launch_image_minmax(const void*, int, int, long long, float*, hipStream_t);
 int launch_image_normalize(const void*, int, int, long long, const float*, float*, hipStream_t);
 int launch_resize_bilinear(const void*, int, float*, int, int, int, int, int, int, hipStream_t);
@@ -370,8 +370,9 @@ int miseg_bn_bwd_sums(const double* stats, int32_t replicas, int32_t stride, int
                       const float* var, float eps, double* sums, void* stream) {
   return launch_bn_bwd_sums(stats, replicas, stride, C, mean, var, eps, sums, (hipStream_t)stream);
 }
-int64_t miseg_group_norm_workspace(int32_t N, int64_t pixels, int32_t C, int32_t backward) {
-  return group_norm_workspace(N, pixels, C, backward);
+int64_t miseg_group_norm_workspace(int32_t N, int64_t pixels, int32_t C, int32_t groups, int32_t dtype, int32_t checkpoint,
+                                   int32_t backward) {
+  return group_norm_workspace(N, pixels, C, groups, dtype, checkpoint, backward);
 }
 int miseg_group_norm_act_fwd(const miseg_group_norm_desc* d, void* stream) {
   MISEG_CHECK_ARG(d, "group_norm_act: null descriptor");

@@ -269,7 +269,8 @@ struct BwdArgs {
   const signed char* codes;
   const bf16_t* scales;
   const float *mean, *rstd, *a, *b, *gamma, *beta; // mean, rstd [N][groups]; a, b [N][C]; gamma, beta [C] (checkpoint)
-  const float *cm, *cp, *cq;                       // [N][C], second pass: dx = a g + (x - cm) cp + cq
+  const float *cm, *cz, *cp, *cq;                  // [N][C], second pass: dx = a g + (x - cm) cp + cq (checkpoint: a g +
+                                                   // xhat cp + cq, z = xhat cm + cz)
   const double2* sums;                             // [N][C], all images: second pass, where the parameters' gradients are due
   float *dgamma, *dbeta;
   long long xps, ximg, dps, dimg, ops, oimg;
@@ -428,7 +429,8 @@ __global__ __launch_bounds__(kNormThreads) void gn_bwd_reduce_kernel(BwdArgs p, 
 // One block per (group, image): the channels' sums over the blocks, then over the group, in 64 bits.
 __global__ __launch_bounds__(kNormThreads) void gn_bwd_finalize_kernel(BwdArgs p, const float2* __restrict__ part, int blocks,
                                                                        int ckpt, double2* __restrict__ sums, float* __restrict__ cm,
-                                                                       float* __restrict__ cp, float* __restrict__ cq) {
+                                                                       float* __restrict__ cz, float* __restrict__ cp,
+                                                                       float* __restrict__ cq) {
   __shared__ double r1[kNormThreads], r2[kNormThreads], lds[4];
   const int w = p.C / p.groups, g = blockIdx.x, n = blockIdx.y;
   const int wide = w < kNormThreads ? w : kNormThreads, lanes = kNormThreads / wide;
@@ -469,8 +471,10 @@ __global__ __launch_bounds__(kNormThreads) void gn_bwd_finalize_kernel(BwdArgs p
   k2 = block_sum(k2, lds) / count;
   const float m = p.mean[n * p.groups + g], rs = p.rstd[n * p.groups + g];
   for (int i = threadIdx.x; i < w; i += kNormThreads) {
-    const long long at = (long long)n * p.C + g * w + i;
-    cm[at] = m;
+    const int c = g * w + i;
+    const long long at = (long long)n * p.C + c;
+    cm[at] = !ckpt ? m : p.gamma ? p.gamma[c] : 1.f;
+    if (ckpt) cz[at] = p.beta ? p.beta[c] : 0.f;
     cp[at] = (float)(ckpt ? -k2 : -k2 * rs);
     cq[at] = (float)-k1;
   }
@@ -503,11 +507,18 @@ __global__ __launch_bounds__(kNormThreads) void gn_bwd_apply_kernel(BwdArgs p) {
   if (!w.active) return;
   float za[8], zb[8], a[8], m[8], kp[8], kq[8];
   const long long cat = (long long)w.n * p.C + w.c;
-  bwd_coef<CK>(za, zb, p, w);
   load_coef(a, p.a + cat);
+  if constexpr (CK) {
+    load_coef(za, p.cm + cat);
+    load_coef(zb, p.cz + cat);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) za[j] = a[j];
+    load_coef(zb, p.b + cat);
+    load_coef(m, p.cm + cat);
+  }
   load_coef(kp, p.cp + cat);
   load_coef(kq, p.cq + cat);
-  if constexpr (!CK) load_coef(m, p.cm + cat);
   BwdFrom<T, CK> from(p, w);
   const int rows = p.g.rows;
   int px = w.p0 + w.r;
@@ -533,6 +544,421 @@ __global__ __launch_bounds__(kNormThreads) void gn_bwd_apply_kernel(BwdArgs p) {
       store8<T, true>(op + u * ostep, pack8<T>(d));
     }
   }
+}
+
+// ------------------------------------------------------------------------------------------------ small maps
+// A block takes all pixels of some groups of one image and keeps them in registers between the statistics and the result:
+// one launch, x read once.  A thread holds up to V pixels of its 8 channels.
+struct SmallGrid {
+  int threads;                                     // per block; 0: the map is too large
+  int slab, slabs;                                 // channels of a block (whole groups, whole 8s), blocks per image
+  int cw, rows;                                    // groups of 8 channels and pixels of a sweep
+};
+constexpr int kSmallThreads[2] = {256, 1024}, kSmallBack[2] = {256, 512};
+
+// Neighbouring slabs share 128-byte lines: blocks 8 apart, which the hardware deals to one chiplet and its L2, take them.
+__device__ __forceinline__ int small_block(int blocks) {
+  const int per = blocks >> 3, b = blockIdx.x;
+  return b < per * 8 ? (b & 7) * per + (b >> 3) : b;
+}
+
+// Threads in segments of `lanes`, a power of two up to 64 or a multiple of 64: the sums over a segment, in its first thread.
+// Every thread of the block calls; `waves` holds one entry per wave.
+struct Segments {
+  int lanes, seg, t;
+  __device__ __forceinline__ Segments(int threads, int segments) {
+    const int most = threads / segments;
+    lanes = most >= 64 ? most & ~63 : 1 << (31 - __clz(most));
+    seg = threadIdx.x / lanes;
+    t = threadIdx.x - seg * lanes;
+  }
+  __device__ __forceinline__ double2 sum(double2 v, double2* waves) const {
+    for (int o = lanes < 64 ? lanes >> 1 : 32; o > 0; o >>= 1) {
+      v.x += __shfl_xor(v.x, o, 64);
+      v.y += __shfl_xor(v.y, o, 64);
+    }
+    if (lanes > 64) {
+      const int wave = threadIdx.x >> 6;
+      if ((threadIdx.x & 63) == 0) waves[wave] = v;
+      __syncthreads();
+      if (t == 0)
+        for (int i = 1; i < lanes >> 6; ++i) {
+          v.x += waves[wave + i].x;
+          v.y += waves[wave + i].y;
+        }
+    }
+    return v;
+  }
+};
+
+// The groups of a thread's 8 channels, the first of them `first` (a multiple of 8 in the slab).
+struct GroupWalk {
+  int g, left, width;
+  __device__ __forceinline__ GroupWalk(int first, int w) : width(w) {
+    g = first / w;
+    left = w - (first - g * w);
+  }
+  __device__ __forceinline__ void next() {
+    if (--left == 0) {
+      left = width;
+      ++g;
+    }
+  }
+};
+
+struct SmallFwdArgs {
+  const char* x;
+  char* y;
+  signed char* codes;
+  bf16_t* scales;
+  const float *gamma, *beta;
+  float *mean, *rstd, *a, *b;
+  long long xps, ximg, yps, yimg;
+  int pixels, C, groups, act, blocks;
+  float eps;
+  SmallGrid g;
+};
+
+template <typename T, int ACT, int V>
+__device__ __forceinline__ void small_fwd_finish(char* yp, long long yps, const Vec8<T> (&v)[V], const float (&a)[8],
+                                                 const float (&b)[8], int r, int rows, int pixels) {
+#pragma unroll
+  for (int u = 0; u < V; ++u) {
+    const int px = r + u * rows;
+    if (px >= pixels) break;
+    float f[8];
+    unpack8(f, v[u]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = act_fwd<ACT>(fmaf(f[j], a[j], b[j]));
+    store8<T>(yp + px * yps * Elem<T>::bytes, pack8<T>(f));
+  }
+}
+
+template <typename T, bool Q, int TB, int V>
+__global__ __launch_bounds__(TB) void gn_small_fwd_kernel(SmallFwdArgs p) {
+  constexpr int ES = Elem<T>::bytes;
+  __shared__ float2 part[TB * 8];
+  __shared__ double2 stat[TB], waves[TB / 64];
+  const int tid = threadIdx.x, id = small_block(p.blocks), n = id / p.g.slabs, c0 = (id - n * p.g.slabs) * p.g.slab;
+  const int channels = p.C - c0 < p.g.slab ? p.C - c0 : p.g.slab, width = p.C / p.groups;
+  const int rows = p.g.rows, cw = p.g.cw, r = tid / cw, l = tid - r * cw, c = c0 + l * 8;
+  const bool active = r < rows && l * 8 < channels;
+  Vec8<T> v[V];
+  const char* xp = p.x + (n * p.ximg + c) * ES;
+#pragma unroll
+  for (int u = 0; u < V; ++u)
+    if (active && r + u * rows < p.pixels) v[u] = load8<T>(xp + (r + u * rows) * p.xps * ES);
+  // pixels of row r: every + (r < over)
+  const int every = p.pixels / rows, over = p.pixels - every * rows;
+  const int bits = width & 7 ? width & 3 ? width & 1 ? 0 : 1 : 2 : 3, merge = 1 << bits;   // channels of a thread in one group
+  if (active) {
+    float k[8], s1[8], s2[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) k[j] = s1[j] = s2[j] = 0.f;
+    if (r < p.pixels) unpack8(k, v[0]);
+#pragma unroll
+    for (int u = 1; u < V; ++u) {
+      if (r + u * rows >= p.pixels) break;
+      float f[8];
+      unpack8(f, v[u]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float d = f[j] - k[j];
+        s1[j] += d;
+        s2[j] = fmaf(d, d, s2[j]);
+      }
+    }
+    // to means and sums of squares around them, then channels of a group joined by twos: equal counts
+    const int count = every + (r < over ? 1 : 0);
+    const float rc = count ? 1.f / (float)count : 0.f;
+    float join = 0.5f * (float)count;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      k[j] += s1[j] * rc;
+      s2[j] -= s1[j] * s1[j] * rc;
+    }
+#pragma unroll
+    for (int size = 1; size < 8; size *= 2)
+      if (merge > size) {
+#pragma unroll
+        for (int j = 0; j < 8; j += 2 * size) {
+          const float d = k[j + size] - k[j];
+          s2[j] += s2[j + size] + d * d * join;
+          k[j] = 0.5f * (k[j] + k[j + size]);
+        }
+        join *= 2.f;
+      }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if ((j & (merge - 1)) == 0) part[tid * (8 >> bits) + (j >> bits)] = make_float2(k[j], s2[j]);
+  }
+  __syncthreads();
+  // the threads' statistics of a group: a row has `entry` of them, each of `merge` channels
+  const int ng = channels / width, entry = width >> bits, pitch = cw * (8 >> bits);
+  const Segments sg(TB, ng);
+  double2 sum = make_double2(0, 0);
+  if (sg.seg < ng) {
+    int row = sg.t / entry, ch = sg.t - row * entry;
+    const int drow = sg.lanes / entry, dch = sg.lanes - drow * entry, last = rows < p.pixels ? rows : p.pixels;
+    while (row < last) {
+      const float2 q = part[row * pitch + sg.seg * entry + ch];
+      const double count = (every + (row < over ? 1 : 0)) * merge, m = q.x;
+      sum.x += count * m;
+      sum.y += (double)q.y + count * m * m;
+      row += drow;
+      ch += dch;
+      if (ch >= entry) {
+        ch -= entry;
+        ++row;
+      }
+    }
+  }
+  sum = sg.sum(sum, waves);
+  if (sg.seg < ng && sg.t == 0) {
+    const double rcount = 1.0 / ((double)p.pixels * width), m = sum.x * rcount;
+    double var = sum.y * rcount - m * m;
+    if (var < 0) var = 0;
+    const double rs = 1.0 / sqrt(var + (double)p.eps);
+    const int at = n * p.groups + c0 / width + sg.seg;
+    p.mean[at] = (float)m;
+    p.rstd[at] = (float)rs;
+    stat[sg.seg] = make_double2(m, rs);
+  }
+  __syncthreads();
+  if (active) {
+    float a[8], b[8];
+    GroupWalk gw(l * 8, width);
+#pragma unroll
+    for (int j = 0; j < 8; ++j, gw.next()) {
+      const double2 q = stat[gw.g];
+      const double sc = p.gamma ? p.gamma[c + j] * q.y : q.y;
+      a[j] = (float)sc;
+      b[j] = (float)((p.beta ? p.beta[c + j] : 0.0) - q.x * sc);
+    }
+    if (r == 0) {
+      float4 *pa = reinterpret_cast<float4*>(p.a + (long long)n * p.C + c), *pb = reinterpret_cast<float4*>(p.b + (long long)n * p.C + c);
+      pa[0] = make_float4(a[0], a[1], a[2], a[3]);
+      pa[1] = make_float4(a[4], a[5], a[6], a[7]);
+      pb[0] = make_float4(b[0], b[1], b[2], b[3]);
+      pb[1] = make_float4(b[4], b[5], b[6], b[7]);
+    }
+    char* yp = p.y + (n * p.yimg + c) * ES;
+    if (p.act == NA_RELU) small_fwd_finish<T, NA_RELU, V>(yp, p.yps, v, a, b, r, rows, p.pixels);
+    else if (p.act == NA_SILU) small_fwd_finish<T, NA_SILU, V>(yp, p.yps, v, a, b, r, rows, p.pixels);
+    else small_fwd_finish<T, NA_NONE, V>(yp, p.yps, v, a, b, r, rows, p.pixels);
+  }
+  if constexpr (Q) {
+    if (r >= rows) return;                        // whole quads of lanes: the others stay for the exchange in quantise8
+    float qs[8], qt[8];
+    GroupWalk gw(active ? l * 8 : 0, width);
+#pragma unroll
+    for (int j = 0; j < 8; ++j, gw.next()) {
+      const double2 q = stat[gw.g < ng ? gw.g : 0];
+      qs[j] = (float)q.y;
+      qt[j] = (float)(-q.x * q.y);
+    }
+    const int blocks32 = (p.C + 31) >> 5;
+#pragma unroll
+    for (int u = 0; u < V; ++u) {
+      const int px = r + u * rows;
+      if (px >= p.pixels) break;
+      float f[8];
+      unpack8(f, v[u]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = active ? fmaf(f[j], qs[j], qt[j]) : 0.f;
+      const Quant8 q = quantise8(f);
+      if (active) {
+        const long long row = (long long)n * p.pixels + px;
+        *reinterpret_cast<uint2*>(p.codes + row * p.C + c) = q.codes;
+        if ((c & 31) == 0) p.scales[row * blocks32 + (c >> 5)] = q.scale;
+      }
+    }
+  }
+}
+
+// Backward: x (or its codes) and dy stay in registers.  One image writes the parameters' gradients, several their sums.
+struct SmallBwdArgs {
+  BwdArgs p;
+  double2* sums;
+  int act, blocks;
+  SmallGrid g;
+};
+
+template <typename T, int ACT, bool CK, int V>
+__device__ __forceinline__ void small_bwd_sums(float (&s1)[8], float (&s2)[8], const BwdLoad<T, CK> (&v)[V],
+                                               const float (&za)[8], const float (&zb)[8], const float (&m)[8], int r, int rows,
+                                               int pixels) {
+#pragma unroll
+  for (int u = 0; u < V; ++u) {
+    if (r + u * rows >= pixels) break;
+    float f[8], d[8];
+    unpack8(d, v[u].dy);
+    if constexpr (CK) dequantise8(f, v[u].codes, bf16_to_f32(v[u].scale));
+    else unpack8(f, v[u].x);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float gj = act_bwd<ACT>(fmaf(f[j], za[j], zb[j]), d[j]);
+      s1[j] += gj;
+      s2[j] = fmaf(gj, CK ? f[j] : f[j] - m[j], s2[j]);
+    }
+  }
+}
+template <typename T, int ACT, bool CK, int V>
+__device__ __forceinline__ void small_bwd_finish(char* op, long long ops, const BwdLoad<T, CK> (&v)[V], const float (&a)[8],
+                                                 const float (&za)[8], const float (&zb)[8], const float (&m)[8],
+                                                 const float (&kp)[8], const float (&kq)[8], int r, int rows, int pixels) {
+  constexpr int ES = Elem<T>::bytes;
+#pragma unroll
+  for (int u = 0; u < V; ++u) {
+    const int px = r + u * rows;
+    if (px >= pixels) break;
+    float f[8], d[8];
+    unpack8(d, v[u].dy);
+    if constexpr (CK) dequantise8(f, v[u].codes, bf16_to_f32(v[u].scale));
+    else unpack8(f, v[u].x);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float gj = act_bwd<ACT>(fmaf(f[j], za[j], zb[j]), d[j]);
+      d[j] = fmaf(a[j], gj, fmaf(CK ? f[j] : f[j] - m[j], kp[j], kq[j]));
+    }
+    store8<T>(op + px * ops * ES, pack8<T>(d));
+  }
+}
+
+template <bool CK>
+__device__ __forceinline__ void small_bwd_coef(float (&za)[8], float (&zb)[8], float (&m)[8], float (&rs)[8], const BwdArgs& p,
+                                               int n, int c, int width) {
+  const long long at = (long long)n * p.C + c;
+  if constexpr (CK) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      za[j] = p.gamma ? p.gamma[c + j] : 1.f;
+      zb[j] = p.beta ? p.beta[c + j] : 0.f;
+      m[j] = 0.f;
+      rs[j] = 1.f;
+    }
+  } else {
+    load_coef(za, p.a + at);
+    load_coef(zb, p.b + at);
+    GroupWalk gw(c, width);
+    gw.g += n * p.groups;
+#pragma unroll
+    for (int j = 0; j < 8; ++j, gw.next()) {
+      m[j] = p.mean[gw.g];
+      rs[j] = p.rstd[gw.g];
+    }
+  }
+}
+
+template <typename T, bool CK, int TB, int V>
+__global__ __launch_bounds__(TB) void gn_small_bwd_kernel(SmallBwdArgs q) {
+  constexpr int ES = Elem<T>::bytes;
+  __shared__ float2 part[TB * 8];
+  __shared__ double2 tree[TB], chan[TB], waves[TB / 64];
+  const BwdArgs& p = q.p;
+  const int tid = threadIdx.x, id = small_block(q.blocks), n = id / q.g.slabs, c0 = (id - n * q.g.slabs) * q.g.slab;
+  const int channels = p.C - c0 < q.g.slab ? p.C - c0 : q.g.slab, width = p.C / p.groups;
+  const int rows = q.g.rows, cw = q.g.cw, r = tid / cw, l = tid - r * cw, c = c0 + l * 8;
+  const bool active = r < rows && l * 8 < channels;
+  BwdLoad<T, CK> v[V];
+  if (active) {
+#pragma unroll
+    for (int u = 0; u < V; ++u) {
+      const int px = r + u * rows;
+      if (px >= p.pixels) break;
+      if constexpr (CK) {
+        const long long row = (long long)n * p.pixels + px;
+        v[u].codes = load_codes<false>(p.codes + row * p.C + c);
+        v[u].scale = p.scales[row * ((p.C + 31) >> 5) + (c >> 5)];
+      } else {
+        v[u].x = load8<T>(p.x + (n * p.ximg + px * p.xps + c) * ES);
+      }
+      v[u].dy = load8<T>(p.dy + (n * p.dimg + px * p.dps + c) * ES);
+    }
+  }
+  if (active) {
+    float za[8], zb[8], m[8], rs[8], s1[8], s2[8];
+    small_bwd_coef<CK>(za, zb, m, rs, p, n, c, width);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s1[j] = s2[j] = 0.f;
+    if (q.act == NA_RELU) small_bwd_sums<T, NA_RELU, CK, V>(s1, s2, v, za, zb, m, r, rows, p.pixels);
+    else if (q.act == NA_SILU) small_bwd_sums<T, NA_SILU, CK, V>(s1, s2, v, za, zb, m, r, rows, p.pixels);
+    else small_bwd_sums<T, NA_NONE, CK, V>(s1, s2, v, za, zb, m, r, rows, p.pixels);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) part[j * TB + tid] = make_float2(s1[j], s2[j] * rs[j]);
+  }
+  __syncthreads();
+  // per channel, by `parts` threads each; slot = j * cw + l
+  const int used = rows < p.pixels ? rows : p.pixels, slots = cw * 8, parts = TB / slots;
+  const int slot = tid % slots, share = tid / slots, sj = slot / cw, sl = slot - sj * cw, ch = sl * 8 + sj;
+  double2 sum = make_double2(0, 0);
+  if (share < parts && ch < channels)
+    for (int row = share; row < used; row += parts) {
+      const float2 e = part[sj * TB + row * cw + sl];
+      sum.x += e.x;
+      sum.y += e.y;
+    }
+  tree[tid] = sum;
+  __syncthreads();
+  for (int left = parts; left > 1;) {
+    const int half = (left + 1) >> 1;
+    if (share + half < left) {
+      tree[tid].x += tree[tid + half * slots].x;
+      tree[tid].y += tree[tid + half * slots].y;
+    }
+    __syncthreads();
+    left = half;
+  }
+  if (tid < slots && ch < channels) {
+    const long long at = (long long)n * p.C + c0 + ch;
+    const double2 e = tree[tid];
+    if (p.images == 1) {
+      if (p.dbeta) p.dbeta[c0 + ch] = (float)e.x;
+      if (p.dgamma) p.dgamma[c0 + ch] = (float)e.y;
+    } else {
+      q.sums[at] = e;
+    }
+    const double sc = p.a[at];
+    chan[ch] = make_double2(sc * e.x, sc * e.y);
+  }
+  __syncthreads();
+  // per group
+  const int ng = channels / width;
+  const Segments sg(TB, ng);
+  sum = make_double2(0, 0);
+  if (sg.seg < ng)
+    for (int e = sg.t; e < width; e += sg.lanes) {
+      sum.x += chan[sg.seg * width + e].x;
+      sum.y += chan[sg.seg * width + e].y;
+    }
+  sum = sg.sum(sum, waves);
+  if (sg.seg < ng && sg.t == 0) tree[sg.seg] = sum;
+  __syncthreads();
+  if (!active) return;
+  const double rcount = 1.0 / ((double)p.pixels * width);
+  float za[8], zb[8], m[8], a[8], kp[8], kq[8];   // read again rather than held over the exchange: registers are short
+  small_bwd_coef<CK>(za, zb, m, kp, p, n, c, width);
+  if constexpr (CK) load_coef(a, p.a + (long long)n * p.C + c);
+  else
+#pragma unroll
+    for (int j = 0; j < 8; ++j) a[j] = za[j];
+  GroupWalk gw(l * 8, width);
+#pragma unroll
+  for (int j = 0; j < 8; ++j, gw.next()) {
+    const double2 k = tree[gw.g];
+    kp[j] = (float)(-k.y * rcount * kp[j]);
+    kq[j] = (float)(-k.x * rcount);
+  }
+  char* op = p.dx + (n * p.oimg + c) * ES;
+  if (q.act == NA_RELU) small_bwd_finish<T, NA_RELU, CK, V>(op, p.ops, v, a, za, zb, m, kp, kq, r, rows, p.pixels);
+  else if (q.act == NA_SILU) small_bwd_finish<T, NA_SILU, CK, V>(op, p.ops, v, a, za, zb, m, kp, kq, r, rows, p.pixels);
+  else small_bwd_finish<T, NA_NONE, CK, V>(op, p.ops, v, a, za, zb, m, kp, kq, r, rows, p.pixels);
+}
+
+__global__ __launch_bounds__(kNormThreads) void gn_bwd_params_kernel(const double2* __restrict__ sums, int images, int C,
+                                                                     float* dgamma, float* dbeta) {
+  const int c = blockIdx.x * kNormThreads + threadIdx.x;
+  if (c < C) gn_bwd_params(sums, images, C, c, dgamma, dbeta);
 }
 
 // ------------------------------------------------------------------------------------------------ launches
@@ -576,6 +1002,42 @@ constexpr int kPassBlocks = 32768, kPassLeast = 4; // the same for a pass that o
 // pass to the second.
 constexpr long long kCacheBytes = 200000000;
 
+// Registers hold V vectors of 8 values a thread in blocks of 256 and 1024 threads.
+template <typename T> struct SmallHold { static constexpr int fwd[2] = {8, 16}, bwd[2] = {4, 16}; };
+template <> struct SmallHold<f32s> { static constexpr int fwd[2] = {4, 8}, bwd[2] = {2, 8}; };
+
+static int gcd_int(int a, int b) { return b ? gcd_int(b, a % b) : a; }
+
+// One launch pays where few pixels meet few channels: a load of a slab narrower than a line keeps a lane for every line, so
+// a block's time grows with its pixels (fp32, 61 x 83 x 40 in slabs of 8: 17 us in one launch, 13 in three; bf16, 30 x 40 x
+// 512 backward: 11 us, 15 in three).  Slabs are the widest of whole groups and whole 8s (32s where 32-channel blocks are
+// written) that a block can hold, up to 64 channels, while 256 blocks are left.
+constexpr int kSmallPixels = 2048;
+static SmallGrid small_grid(long long N, long long pixels, int C, int groups, bool whole32, const int (&threads)[2],
+                            const int (&hold)[2]) {
+  SmallGrid g{};
+  if (pixels > kSmallPixels) return g;
+  const int width = C / groups, whole = whole32 ? 32 : 8;
+  long long unit = (long long)width / gcd_int(width, whole) * whole;
+  if (unit > C) unit = C;
+  auto columns = [&](long long slab) { return whole32 ? (slab + 31) / 32 * 4 : slab / 8; };
+  auto fits = [&](long long slab, int k) {
+    if (columns(slab) * 8 > threads[k]) return false;
+    const long long rows = threads[k] / columns(slab);
+    return (pixels + rows - 1) / rows <= hold[k];
+  };
+  auto blocks = [&](long long slab) { return N * ((C + slab - 1) / slab); };
+  if (!fits(unit, 0) && !fits(unit, 1)) return g;
+  long long slab = unit;
+  while (slab * 2 <= C && slab * 2 <= 64 && (fits(slab * 2, 0) || fits(slab * 2, 1)) && blocks(slab * 2) >= 256) slab *= 2;
+  g.threads = threads[fits(slab, 0) ? 0 : 1];
+  g.slab = (int)slab;
+  g.slabs = (int)((C + slab - 1) / slab);
+  g.cw = (int)columns(slab);
+  g.rows = g.threads / g.cw;
+  return g;
+}
+
 static int images_per_step(long long N, long long image_bytes) {
   const long long n = kCacheBytes / image_bytes;
   return (int)(n < 1 ? 1 : n < N ? n : N);
@@ -592,9 +1054,20 @@ static long long gn_partials(long long N, long long pixels, int C) {
   return round_up(slab * (blocks < most ? blocks : most));
 }
 
-static long long gn_workspace(long long N, long long pixels, int C, int backward) {
-  const long long part = gn_partials(N, pixels, C), coef = round_up(4LL * N * C);
-  return backward ? part + 2 * round_up(8LL * N * C) + 3 * coef : part + 2 * coef;
+static SmallGrid small_fwd(long long N, long long pixels, int C, int groups, int dtype, bool checkpoint) {
+  const int (&hold)[2] = dtype == MISEG_DT_F32 ? SmallHold<f32s>::fwd : SmallHold<bf16s>::fwd;
+  return small_grid(N, pixels, C, groups, checkpoint, kSmallThreads, hold);
+}
+static SmallGrid small_bwd(long long N, long long pixels, int C, int groups, int dtype) {
+  const int (&hold)[2] = dtype == MISEG_DT_F32 ? SmallHold<f32s>::bwd : SmallHold<bf16s>::bwd;
+  return small_grid(N, pixels, C, groups, false, kSmallBack, hold);
+}
+
+static long long gn_workspace(long long N, long long pixels, int C, int groups, int dtype, int checkpoint, int backward) {
+  const long long part = gn_partials(N, pixels, C), coef = round_up(4LL * N * C), sums = 2 * round_up(8LL * N * C);
+  if (!backward) return small_fwd(N, pixels, C, groups, dtype, checkpoint).threads ? 0 : part + (checkpoint ? 2 * coef : 0);
+  if (small_bwd(N, pixels, C, groups, dtype).threads) return N > 1 ? sums : 0;
+  return sums + part + 4 * coef;
 }
 
 static void launch_pass(const PassArgs& p, int N, int storage, int act, hipStream_t s) {
@@ -623,11 +1096,31 @@ int launch_group_norm_fwd(const miseg_group_norm_desc* d, hipStream_t s) {
   MISEG_CHECK_ARG(d->eps >= 0.f, "group_norm_act: eps = %g", (double)d->eps);
   MISEG_CHECK_ARG(!d->codes == !d->code_scales && ((uintptr_t)d->codes & 7) == 0 && ((uintptr_t)d->code_scales & 1) == 0,
                   "group_norm_act: codes and code_scales go together, 8-byte and 2-byte aligned");
-  const long long need = gn_workspace(d->N, d->pixels, d->C, 0);
-  MISEG_CHECK_ARG(d->workspace && good_coef(d->workspace) && d->workspace_bytes >= need,
+  const long long need = gn_workspace(d->N, d->pixels, d->C, d->groups, d->dtype, d->codes != nullptr, 0);
+  MISEG_CHECK_ARG(!need || (d->workspace && good_coef(d->workspace) && d->workspace_bytes >= need),
                   "group_norm_act: the workspace must be 16-byte aligned and hold %lld bytes (%lld given)", need,
                   (long long)d->workspace_bytes);
   const int storage = storage_of(d->dtype, d->fmt);
+  const SmallGrid sg = small_fwd(d->N, d->pixels, d->C, d->groups, d->dtype, d->codes != nullptr);
+  if (sg.threads) {
+    SmallFwdArgs p{(const char*)d->x, (char*)d->y, (signed char*)d->codes, (bf16_t*)d->code_scales, d->gamma, d->beta,
+                   d->mean, d->rstd, d->scale, d->shift, d->x_pix, d->x_img, d->y_pix, d->y_img, (int)d->pixels, d->C,
+                   d->groups, act_of(d->act), d->N * sg.slabs, d->eps, sg};
+    const dim3 grid(p.blocks), block(sg.threads);
+    by_type_act(storage, NA_NONE, [&](auto t, auto) {
+      typedef decltype(t) T;
+      typedef SmallHold<T> H;
+      if (sg.threads == kSmallThreads[0]) {
+        if (d->codes) hipLaunchKernelGGL((gn_small_fwd_kernel<T, true, kSmallThreads[0], H::fwd[0]>), grid, block, 0, s, p);
+        else hipLaunchKernelGGL((gn_small_fwd_kernel<T, false, kSmallThreads[0], H::fwd[0]>), grid, block, 0, s, p);
+      } else {
+        if (d->codes) hipLaunchKernelGGL((gn_small_fwd_kernel<T, true, kSmallThreads[1], H::fwd[1]>), grid, block, 0, s, p);
+        else hipLaunchKernelGGL((gn_small_fwd_kernel<T, false, kSmallThreads[1], H::fwd[1]>), grid, block, 0, s, p);
+      }
+    });
+    MISEG_CHECK_HIP(hipGetLastError());
+    return MISEG_OK;
+  }
   char* ws = (char*)d->workspace;
   float2* part = (float2*)ws;
   ws += gn_partials(d->N, d->pixels, d->C);
@@ -679,19 +1172,44 @@ int launch_group_norm_bwd(const miseg_group_norm_bwd_desc* d, hipStream_t s) {
                   "group_norm_act_bwd: dx overlaps x or dy without being it or another channel range of its buffer");
   MISEG_CHECK_ARG(d->mean && d->rstd && d->scale && d->shift && good_coef(d->scale) && good_coef(d->shift),
                   "group_norm_act_bwd: mean, rstd, scale and shift are needed, scale and shift 16-byte aligned");
-  const long long need = gn_workspace(d->N, d->pixels, d->C, 1);
-  MISEG_CHECK_ARG(d->workspace && good_coef(d->workspace) && d->workspace_bytes >= need,
+  const long long need = gn_workspace(d->N, d->pixels, d->C, d->groups, d->dtype, d->codes != nullptr, 1);
+  MISEG_CHECK_ARG(!need || (d->workspace && good_coef(d->workspace) && d->workspace_bytes >= need),
                   "group_norm_act_bwd: the workspace must be 16-byte aligned and hold %lld bytes (%lld given)", need,
                   (long long)d->workspace_bytes);
   const int storage = storage_of(d->dtype, d->fmt), act = act_of(d->act);
   const bool ck = d->codes != nullptr;
   char* ws = (char*)d->workspace;
+  double2* sums = (double2*)ws;
+  const SmallGrid sg = small_bwd(d->N, d->pixels, d->C, d->groups, d->dtype);
+  if (sg.threads) {
+    SmallBwdArgs q{{(const char*)d->x, (const char*)d->dy, (char*)d->dx, (const signed char*)d->codes,
+                    (const bf16_t*)d->code_scales, d->mean, d->rstd, d->scale, d->shift, d->gamma, d->beta, nullptr, nullptr,
+                    nullptr, nullptr, nullptr, d->dgamma, d->dbeta, d->x_pix, d->x_img, d->dy_pix, d->dy_img, d->dx_pix,
+                    d->dx_img, (int)d->pixels, d->C, d->groups, d->N, NormGrid{}},
+                   sums, act, d->N * sg.slabs, sg};
+    const dim3 grid(q.blocks), block(sg.threads);
+    by_type_act(storage, NA_NONE, [&](auto t, auto) {
+      typedef decltype(t) T;
+      typedef SmallHold<T> H;
+      if (sg.threads == kSmallBack[0]) {
+        if (ck) hipLaunchKernelGGL((gn_small_bwd_kernel<T, true, kSmallBack[0], H::bwd[0]>), grid, block, 0, s, q);
+        else hipLaunchKernelGGL((gn_small_bwd_kernel<T, false, kSmallBack[0], H::bwd[0]>), grid, block, 0, s, q);
+      } else {
+        if (ck) hipLaunchKernelGGL((gn_small_bwd_kernel<T, true, kSmallBack[1], H::bwd[1]>), grid, block, 0, s, q);
+        else hipLaunchKernelGGL((gn_small_bwd_kernel<T, false, kSmallBack[1], H::bwd[1]>), grid, block, 0, s, q);
+      }
+    });
+    if (d->N > 1 && (d->dgamma || d->dbeta))
+      hipLaunchKernelGGL(gn_bwd_params_kernel, dim3((d->C + kNormThreads - 1) / kNormThreads), dim3(kNormThreads), 0, s, sums,
+                         d->N, d->C, d->dgamma, d->dbeta);
+    MISEG_CHECK_HIP(hipGetLastError());
+    return MISEG_OK;
+  }
+  ws += 2 * round_up(8LL * d->N * d->C);
   float2* part = (float2*)ws;
   ws += gn_partials(d->N, d->pixels, d->C);
-  double2* sums = (double2*)ws;
-  ws += 2 * round_up(8LL * d->N * d->C);
   const long long coef = round_up(4LL * d->N * d->C);
-  float *cm = (float*)ws, *cp = (float*)(ws + coef), *cq = (float*)(ws + 2 * coef);
+  float *cm = (float*)ws, *cz = (float*)(ws + coef), *cp = (float*)(ws + 2 * coef), *cq = (float*)(ws + 3 * coef);
   const long long dbytes = d->pixels * d->C * bytes, xbytes = ck ? d->pixels * (d->C + 2 * ((d->C + 31) / 32)) : dbytes;
   // both stay in the cache if they can; else dy alone; else the last pixels of both
   const bool alone = xbytes + dbytes > kCacheBytes && dbytes <= kCacheBytes;
@@ -701,7 +1219,7 @@ int launch_group_norm_bwd(const miseg_group_norm_bwd_desc* d, hipStream_t s) {
     const long long cat = (long long)n0 * d->C, gat = (long long)n0 * d->groups;
     BwdArgs p{(const char*)d->x + n0 * d->x_img * bytes, (const char*)d->dy + n0 * d->dy_img * bytes,
               (char*)d->dx + n0 * d->dx_img * bytes, (const signed char*)d->codes, (const bf16_t*)d->code_scales,
-              d->mean + gat, d->rstd + gat, d->scale + cat, d->shift + cat, d->gamma, d->beta, cm, cp, cq, nullptr,
+              d->mean + gat, d->rstd + gat, d->scale + cat, d->shift + cat, d->gamma, d->beta, cm, cz, cp, cq, nullptr,
               d->dgamma, d->dbeta, d->x_pix, d->x_img, d->dy_pix, d->dy_img, d->dx_pix, d->dx_img, (int)d->pixels, d->C,
               d->groups, d->N, norm_grid(n, d->pixels, d->C, kStatBlocks, kStatLeast)};
     if (ck) {
@@ -719,7 +1237,7 @@ int launch_group_norm_bwd(const miseg_group_norm_bwd_desc* d, hipStream_t s) {
       else hipLaunchKernelGGL((gn_bwd_reduce_kernel<T, A, false, false>), grid, dim3(kNormThreads), 0, s, p, part);
     });
     hipLaunchKernelGGL(gn_bwd_finalize_kernel, dim3(d->groups, n), dim3(kNormThreads), 0, s, p, part, blocks, ck ? 1 : 0,
-                       sums + cat, cm, cp, cq);
+                       sums + cat, cm, cz, cp, cq);
     p.g = norm_grid(n, d->pixels, d->C, kPassBlocks, kPassLeast);
     const bool params = n0 + n == d->N && (d->dgamma || d->dbeta);
     if (params) p.sums = sums;
@@ -780,12 +1298,13 @@ int launch_checkpoint8_read(const miseg_checkpoint8_desc* d, hipStream_t s) {
   return MISEG_OK;
 }
 
-long long group_norm_workspace(int N, long long pixels, int C, int backward) {
-  if (N <= 0 || N > 65535 || pixels <= 0 || pixels >= (1LL << 31) / 4 || C <= 0 || (C & 7) || C > 65536) {
-    set_error("group_norm_workspace: N = %d, pixels = %lld, C = %d", N, pixels, C);
+long long group_norm_workspace(int N, long long pixels, int C, int groups, int dtype, int checkpoint, int backward) {
+  if (N <= 0 || N > 65535 || pixels <= 0 || pixels >= (1LL << 31) / 4 || C <= 0 || (C & 7) || C > 65536 || groups <= 0 ||
+      C % groups || (dtype != MISEG_DT_BF16 && dtype != MISEG_DT_F32)) {
+    set_error("group_norm_workspace: N = %d, pixels = %lld, C = %d, groups = %d, dtype = %d", N, pixels, C, groups, dtype);
     return MISEG_E_INVALID_ARG;
   }
-  return gn_workspace(N, pixels, C, backward);
+  return gn_workspace(N, pixels, C, groups, dtype, checkpoint, backward);
 }
 
 }  // namespace miseg

@@ -185,7 +185,7 @@ SIGNATURES = {
     "miseg_bn_bwd_sums": (C.c_int, [_VP, _I32, _I32, _I32, _FP, _FP, C.c_float, _VP, _VP]),
     "miseg_bn_relu_bwd_apply": (C.c_int, [_VP, _VP, _VP, _I64, _I32, _I32, _I32, _I32, _FP, _FP, _FP,
                                           _FP, C.c_float, _I32, _VP, _VP, _I32, _VP]),
-    "miseg_group_norm_workspace": (C.c_int64, [_I32, _I64, _I32, _I32]),
+    "miseg_group_norm_workspace": (C.c_int64, [_I32, _I64, _I32, _I32, _I32, _I32, _I32]),
     "miseg_group_norm_act_fwd": (C.c_int, [C.POINTER(GroupNormDesc), _VP]),
     "miseg_group_norm_act_bwd": (C.c_int, [C.POINTER(GroupNormBwdDesc), _VP]),
     "miseg_checkpoint8_write": (C.c_int, [C.POINTER(Checkpoint8Desc), _VP]),

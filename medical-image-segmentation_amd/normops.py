@@ -31,6 +31,15 @@ class Checkpoint8:
             raise L.MisegError("the codes and scales of a checkpoint are dense and on one device")
         self.codes, self.scales = codes, scales
 
+    @classmethod
+    def _like(cls, x):
+        """An unwritten checkpoint for a tensor that `_view` has accepted."""
+        self = cls.__new__(cls)
+        n, h, w, c = x.shape
+        self.codes = x.new_empty((n, h, w, c), dtype=torch.int8)
+        self.scales = x.new_empty((n, h, w, (c + 31) // 32), dtype=torch.bfloat16)
+        return self
+
     @property
     def shape(self):
         return self.codes.shape
@@ -44,32 +53,51 @@ class Checkpoint8:
 
 
 class Saved:
-    """What `group_norm_act_backward` takes of a forward call: x or its checkpoint, the statistics (N, groups), the
-    coefficients of z = x * scale + shift (N, C), and the layer's parameters."""
+    """What `group_norm_act_backward` takes of a forward call: x or its checkpoint, the statistics `mean` and `rstd`
+    (N, groups), the coefficients of z = x * scale + shift (N, C), and the layer's parameters."""
 
     def __init__(self, x, checkpoint, mean, rstd, scale, shift, gamma, beta, groups, act):
         self.x, self.checkpoint = x, checkpoint
-        self.mean, self.rstd, self.scale, self.shift = mean, rstd, scale, shift
+        self.stats, self.coefs = (mean, rstd), (scale, shift)
         self.gamma, self.beta, self.groups, self.act = gamma, beta, groups, act
+
+    # `stats` and `coefs` are pairs, or tensors with one more dimension that are taken apart only where somebody asks
+    @property
+    def mean(self):
+        return self.stats[0]
+
+    @property
+    def rstd(self):
+        return self.stats[1]
+
+    @property
+    def scale(self):
+        return self.coefs[0]
+
+    @property
+    def shift(self):
+        return self.coefs[1]
 
 
 def _view(t, name, like=None):
     """(pixel stride, image stride) of a channels-last tensor or channel slice."""
     if not isinstance(t, torch.Tensor) or t.dim() != 4 or t.dtype not in _TYPES:
         raise L.MisegError("%s has to be a (N, H, W, C) tensor in bfloat16, float16 or float32" % name)
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise L.MisegError("%s is on %s: these operators run on the GPU" % (name, t.device))
     if like is not None and (t.shape != like.shape or t.device != like.device):
         raise L.MisegError("%s is %s on %s, not %s on %s" % (name, tuple(t.shape), t.device, tuple(like.shape), like.device))
     n, h, w, c = t.shape
     if t.numel() == 0:
         raise L.MisegError("%s is empty: %s" % (name, tuple(t.shape)))
+    if t.is_contiguous():
+        return c, h * w * c
     sn, sh, sw, sc = t.stride()
     pix = sw if w > 1 else sh if h > 1 else max(sw, c)
     if (c > 1 and sc != 1) or (w > 1 and h > 1 and sh != w * pix) or pix < c or (n > 1 and sn < (h * w - 1) * pix + c):
         raise L.MisegError("%s is not channels last: shape %s, strides %s" % (name, tuple(t.shape), t.stride()))
-    per = 16 // t.element_size()
     if h == 1 and w == 1:
+        per = 16 // t.element_size()
         pix = (c + per - 1) // per * per                     # one pixel: its stride is never used
     return pix, sn if n > 1 else h * w * pix
 
@@ -77,9 +105,9 @@ def _view(t, name, like=None):
 def _coef(t, name, shape, device, optional=True):
     if t is None and optional:
         return None
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or tuple(t.shape) != tuple(shape) or \
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or tuple(t.shape) != shape or \
             t.device != device or not t.is_contiguous():
-        raise L.MisegError("%s has to be a dense float32 tensor %s on %s" % (name, tuple(shape), device))
+        raise L.MisegError("%s has to be a dense float32 tensor %s on %s" % (name, shape, device))
     return t.data_ptr()
 
 
@@ -89,17 +117,33 @@ def _act(act):
     return ACTS[act]
 
 
-def _workspace(lib, n, pixels, c, backward, device):
-    size = lib.miseg_group_norm_workspace(n, pixels, c, backward)
+def _groups(groups, c):
+    if not isinstance(groups, int) or groups < 1 or c % groups:
+        raise L.MisegError("%d channels in %r groups" % (c, groups))
+
+
+def _launch(fn, d, device):
+    """fn on the current stream of `device`, whichever device is current."""
+    index = device.index
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(C.byref(d), stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(C.byref(d), stream)
+    if rc:
+        L.check(rc)
+
+
+def _workspace(lib, d, checkpoint, backward, x):
+    size = lib.miseg_group_norm_workspace(d.N, d.pixels, d.C, d.groups, d.dtype, checkpoint, backward)
     if size < 0:
         L.check(int(size))
-    return torch.empty(size, dtype=torch.uint8, device=device)
-
-
-def _new_checkpoint(shape, device):
-    n, h, w, c = shape
-    return Checkpoint8(torch.empty((n, h, w, c), dtype=torch.int8, device=device),
-                       torch.empty((n, h, w, (c + 31) // 32), dtype=torch.bfloat16, device=device))
+    if size == 0:
+        return None
+    ws = x.new_empty(size, dtype=torch.uint8)
+    d.workspace, d.workspace_bytes = ws.data_ptr(), size
+    return ws
 
 
 def group_norm_act(x, gamma, beta, groups, eps=1e-3, act="none", out=None, checkpoint=False):
@@ -108,85 +152,100 @@ def group_norm_act(x, gamma, beta, groups, eps=1e-3, act="none", out=None, check
     out: where y goes, a view like x (x itself only with `checkpoint`).  checkpoint: keep the normalised x in 8 bits, not x.
     Returns y and the `Saved` that the backward pass takes."""
     lib = L.load()
-    x_pix, x_img = _view(x, "x")
-    n, h, w, c = x.shape
-    device = x.device
-    y = torch.empty((n, h, w, c), dtype=x.dtype, device=device) if out is None else out
-    y_pix, y_img = _view(y, "out", x)
-    if y.dtype != x.dtype:
-        raise L.MisegError("out is %s, x %s" % (y.dtype, x.dtype))
-    if y.data_ptr() == x.data_ptr() and not checkpoint:
-        raise L.MisegError("out is x, which the backward pass needs: pass checkpoint=True or another tensor")
-    if not isinstance(groups, int) or groups < 1 or c % groups:
-        raise L.MisegError("%d channels in %r groups" % (c, groups))
-    stats = torch.empty(2 * n * (groups + c) + 8, dtype=torch.float32, device=device)
-    scale, shift = stats[:n * c].view(n, c), stats[n * c:2 * n * c].view(n, c)
-    mean, rstd = stats[2 * n * c:2 * n * c + n * groups].view(n, groups), stats[2 * n * c + n * groups:2 * n * (c + groups)].view(n, groups)
-    ck = _new_checkpoint(x.shape, device) if checkpoint else None
     d = L.GroupNormDesc()
-    d.x, d.y, d.x_pix, d.x_img, d.y_pix, d.y_img = x.data_ptr(), y.data_ptr(), x_pix, x_img, y_pix, y_img
+    d.x_pix, d.x_img = _view(x, "x")
+    n, h, w, c = x.shape
+    device, dtype = x.device, x.dtype
+    _groups(groups, c)
+    d.x = x.data_ptr()
+    if out is None:
+        y = x.new_empty((n, h, w, c))
+        d.y_pix, d.y_img = c, h * w * c
+    else:
+        y = out
+        d.y_pix, d.y_img = _view(y, "out", x)
+        if y.dtype != dtype:
+            raise L.MisegError("out is %s, x %s" % (y.dtype, dtype))
+        if y.data_ptr() == d.x and not checkpoint:
+            raise L.MisegError("out is x, which the backward pass needs: pass checkpoint=True or another tensor")
+    d.y = y.data_ptr()
+    stats, coefs = x.new_empty((2, n, groups), dtype=torch.float32), x.new_empty((2, n, c), dtype=torch.float32)
     d.gamma, d.beta = _coef(gamma, "gamma", (c,), device), _coef(beta, "beta", (c,), device)
-    d.mean, d.rstd, d.scale, d.shift = mean.data_ptr(), rstd.data_ptr(), scale.data_ptr(), shift.data_ptr()
-    if ck is not None:
+    d.mean = at = stats.data_ptr()
+    d.rstd = at + 4 * n * groups
+    d.scale = at = coefs.data_ptr()
+    d.shift = at + 4 * n * c
+    ck = None
+    if checkpoint:
+        ck = Checkpoint8._like(x)
         d.codes, d.code_scales = ck.codes.data_ptr(), ck.scales.data_ptr()
     d.N, d.C, d.groups, d.pixels, d.eps, d.act = n, c, groups, h * w, eps, _act(act)
-    d.dtype, d.fmt = _TYPES[x.dtype]
-    with torch.cuda.device(device):
-        ws = _workspace(lib, n, h * w, c, 0, device)
-        d.workspace, d.workspace_bytes = ws.data_ptr(), ws.numel()
-        L.check(lib.miseg_group_norm_act_fwd(C.byref(d), torch.cuda.current_stream(device).cuda_stream))
-    return y, Saved(None if checkpoint else x, ck, mean, rstd, scale, shift, gamma, beta, groups, act)
+    d.dtype, d.fmt = _TYPES[dtype]
+    ws = _workspace(lib, d, 1 if checkpoint else 0, 0, x)    # noqa: F841: lives until the launch is in its stream
+    _launch(lib.miseg_group_norm_act_fwd, d, device)
+    saved = Saved(None if checkpoint else x, ck, None, None, None, None, gamma, beta, groups, act)
+    saved.stats, saved.coefs = stats, coefs
+    return y, saved
+
+
+def _pair_of(t, names, shape, device):
+    """Addresses of the two tensors of Saved.stats or Saved.coefs."""
+    if isinstance(t, torch.Tensor):
+        at = _coef(t, names[0], (2,) + shape, device, False)
+        return at, at + 4 * shape[0] * shape[1]
+    return _coef(t[0], names[0], shape, device, False), _coef(t[1], names[1], shape, device, False)
 
 
 def group_norm_act_backward(dy, saved, out=None):
     """dx, dgamma and dbeta (float32 (C,)) of `group_norm_act` from the gradient of its result and what it saved.  out: where
     dx goes, a view like dy (dy itself allowed)."""
     lib = L.load()
-    dy_pix, dy_img = _view(dy, "dy")
-    n, h, w, c = dy.shape
-    device, groups = dy.device, saved.groups
-    if (saved.x is None) == (saved.checkpoint is None):
-        raise L.MisegError("the backward pass takes x or its checkpoint")
-    dx = torch.empty((n, h, w, c), dtype=dy.dtype, device=device) if out is None else out
     d = L.GroupNormBwdDesc()
-    d.dx_pix, d.dx_img = _view(dx, "out", dy)
-    if saved.x is not None:
+    d.dy_pix, d.dy_img = _view(dy, "dy")
+    n, h, w, c = dy.shape
+    device, dtype, groups, ck = dy.device, dy.dtype, saved.groups, saved.checkpoint
+    if (saved.x is None) == (ck is None):
+        raise L.MisegError("the backward pass takes x or its checkpoint")
+    _groups(groups, c)
+    d.dy = dy.data_ptr()
+    if ck is None:
         d.x_pix, d.x_img = _view(saved.x, "x", dy)
         d.x = saved.x.data_ptr()
-        if saved.x.dtype != dy.dtype:
-            raise L.MisegError("dy is %s, x %s" % (dy.dtype, saved.x.dtype))
+        if saved.x.dtype != dtype:
+            raise L.MisegError("dy is %s, x %s" % (dtype, saved.x.dtype))
     else:
-        ck = saved.checkpoint
         if ck.shape != dy.shape or ck.device != device:
             raise L.MisegError("the checkpoint is %s on %s, dy %s on %s" % (tuple(ck.shape), ck.device, tuple(dy.shape), device))
         d.codes, d.code_scales = ck.codes.data_ptr(), ck.scales.data_ptr()
-    if dx.dtype != dy.dtype:
-        raise L.MisegError("out is %s, dy %s" % (dx.dtype, dy.dtype))
-    if not isinstance(groups, int) or groups < 1 or c % groups:
-        raise L.MisegError("%d channels in %r groups" % (c, groups))
-    d.mean = _coef(saved.mean, "mean", (n, groups), device, False)
-    d.rstd = _coef(saved.rstd, "rstd", (n, groups), device, False)
-    d.scale = _coef(saved.scale, "scale", (n, c), device, False)
-    d.shift = _coef(saved.shift, "shift", (n, c), device, False)
+    if out is None:
+        dx = dy.new_empty((n, h, w, c))
+        d.dx_pix, d.dx_img = c, h * w * c
+    else:
+        dx = out
+        d.dx_pix, d.dx_img = _view(dx, "out", dy)
+        if dx.dtype != dtype:
+            raise L.MisegError("out is %s, dy %s" % (dx.dtype, dtype))
+    d.dx = dx.data_ptr()
+    d.mean, d.rstd = _pair_of(saved.stats, ("mean", "rstd"), (n, groups), device)
+    d.scale, d.shift = _pair_of(saved.coefs, ("scale", "shift"), (n, c), device)
     d.gamma, d.beta = _coef(saved.gamma, "gamma", (c,), device), _coef(saved.beta, "beta", (c,), device)
-    grads = torch.empty((2, c), dtype=torch.float32, device=device)
-    d.dgamma, d.dbeta = grads[0].data_ptr(), grads[1].data_ptr()
-    d.dy, d.dx, d.dy_pix, d.dy_img = dy.data_ptr(), dx.data_ptr(), dy_pix, dy_img
+    grads = dy.new_empty((2, c), dtype=torch.float32)
+    d.dgamma = at = grads.data_ptr()
+    d.dbeta = at + 4 * c
     d.N, d.C, d.groups, d.pixels, d.act = n, c, groups, h * w, _act(saved.act)
-    d.dtype, d.fmt = _TYPES[dy.dtype]
-    with torch.cuda.device(device):
-        ws = _workspace(lib, n, h * w, c, 1, device)
-        d.workspace, d.workspace_bytes = ws.data_ptr(), ws.numel()
-        L.check(lib.miseg_group_norm_act_bwd(C.byref(d), torch.cuda.current_stream(device).cuda_stream))
-    return dx, grads[0], grads[1]
+    d.dtype, d.fmt = _TYPES[dtype]
+    ws = _workspace(lib, d, 0 if ck is None else 1, 1, dy)   # noqa: F841
+    _launch(lib.miseg_group_norm_act_bwd, d, device)
+    dgamma, dbeta = grads.unbind(0)
+    return dx, dgamma, dbeta
 
 
 def _pair(a, b, what, n, c, device):
     """Coefficients (C,) or (N, C) as (pointer, pointer, elements from one image's to the next's)."""
-    if (a is None) != (b is None):
-        raise L.MisegError("%s: a scale and a shift go together" % what)
-    if a is None:
+    if a is None and b is None:
         return None, None, 0
+    if a is None or b is None:
+        raise L.MisegError("%s: a scale and a shift go together" % what)
     shape = (n, c) if a.dim() == 2 else (c,)
     return _coef(a, what + " scale", shape, device), _coef(b, what + " shift", shape, device), c if a.dim() == 2 else 0
 
@@ -195,46 +254,46 @@ def checkpoint8_write(x, scale=None, shift=None, y_scale=None, y_shift=None, act
     """The 8-bit checkpoint of x, or of x * scale + shift with float32 coefficients (C,) or (N, C).  With y_scale and y_shift
     also y = act(x * y_scale + y_shift) of the same pass, into `out` if given (x itself allowed): returns (checkpoint, y)."""
     lib = L.load()
-    x_pix, x_img = _view(x, "x")
-    n, h, w, c = x.shape
     d = L.Checkpoint8Desc()
-    d.x, d.x_pix, d.x_img = x.data_ptr(), x_pix, x_img
-    d.code_a, d.code_b, img = _pair(scale, shift, "code", n, c, x.device)
-    d.y_a, d.y_b, y_of = _pair(y_scale, y_shift, "y", n, c, x.device)
+    d.x_pix, d.x_img = _view(x, "x")
+    n, h, w, c = x.shape
+    device = x.device
+    d.x = x.data_ptr()
+    d.code_a, d.code_b, img = _pair(scale, shift, "code", n, c, device)
+    d.y_a, d.y_b, y_of = _pair(y_scale, y_shift, "y", n, c, device)
     if scale is not None and y_scale is not None and img != y_of:
         raise L.MisegError("the coefficients of the codes and of y are both (C,) or both (N, C)")
     d.coef_img = max(img, y_of)
     y = None
     if y_scale is not None:
-        y = torch.empty((n, h, w, c), dtype=x.dtype, device=x.device) if out is None else out
+        y = x.new_empty((n, h, w, c)) if out is None else out
         if y.dtype != x.dtype:
             raise L.MisegError("out is %s, x %s" % (y.dtype, x.dtype))
         d.y_pix, d.y_img = _view(y, "out", x)
         d.y = y.data_ptr()
     elif out is not None or act != "none":
         raise L.MisegError("an activation and out belong to y, which takes y_scale and y_shift")
-    ck = _new_checkpoint(x.shape, x.device)
+    ck = Checkpoint8._like(x)
     d.codes, d.code_scales = ck.codes.data_ptr(), ck.scales.data_ptr()
     d.N, d.C, d.pixels, d.act = n, c, h * w, _act(act)
     d.dtype, d.fmt = _TYPES[x.dtype]
-    with torch.cuda.device(x.device):
-        L.check(lib.miseg_checkpoint8_write(C.byref(d), torch.cuda.current_stream(x.device).cuda_stream))
+    _launch(lib.miseg_checkpoint8_write, d, device)
     return ck if y is None else (ck, y)
 
 
 def checkpoint8_read(checkpoint, scale=None, shift=None, act="none", dtype=torch.bfloat16, out=None):
     """act(v * scale + shift) of a checkpoint's values v as a tensor of `dtype` (of out's type where it is given)."""
     lib = L.load()
-    n, h, w, c = checkpoint.shape
-    device = checkpoint.device
+    codes = checkpoint.codes
+    n, h, w, c = codes.shape
+    device = codes.device
     if out is None:
-        out = torch.empty((n, h, w, c), dtype=dtype, device=device)
+        out = codes.new_empty((n, h, w, c), dtype=dtype)
     d = L.Checkpoint8Desc()
     d.y_pix, d.y_img = _view(out, "out", checkpoint)
-    d.y, d.codes, d.code_scales = out.data_ptr(), checkpoint.codes.data_ptr(), checkpoint.scales.data_ptr()
+    d.y, d.codes, d.code_scales = out.data_ptr(), codes.data_ptr(), checkpoint.scales.data_ptr()
     d.y_a, d.y_b, d.coef_img = _pair(scale, shift, "y", n, c, device)
     d.N, d.C, d.pixels, d.act = n, c, h * w, _act(act)
     d.dtype, d.fmt = _TYPES[out.dtype]
-    with torch.cuda.device(device):
-        L.check(lib.miseg_checkpoint8_read(C.byref(d), torch.cuda.current_stream(device).cuda_stream))
+    _launch(lib.miseg_checkpoint8_read, d, device)
     return out

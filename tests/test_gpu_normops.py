@@ -177,9 +177,9 @@ def test_checkpoint_of_the_forward_pass_and_backward_out_of_it(ops, shape, dt):
     n, h, w, c, groups = shape
     for act in ("relu", "silu"):
         x, dy, gamma, beta = make(n, h, w, c, dt, seed=3 * c + w)
-        plain, kept = ops.group_norm_act(x, gamma, beta, groups, act=act)
         y, saved = ops.group_norm_act(x, gamma, beta, groups, act=act, checkpoint=True)
-        assert torch.equal(y, plain) and torch.equal(saved.mean, kept.mean) and saved.x is None
+        check_forward(x, y, saved, gamma, beta, groups, 1e-3, act)
+        assert saved.x is None
         mean, rstd, scale, _ = stats64(x, gamma, beta, groups, 1e-3)
         xhat = (x.double() - spread(mean, c)) * spread(rstd, c)
         xmax = spread(x.double().abs().amax((1, 2)).reshape(n, groups, -1).amax(2), c)

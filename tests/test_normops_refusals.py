@@ -22,7 +22,7 @@ def fwd(**kw):
     d = L.GroupNormDesc()
     for i, f in enumerate(("x", "y", "mean", "rstd", "scale", "shift", "workspace")):
         setattr(d, f, A + (i << 24))
-    d.N, d.C, d.groups, d.pixels, d.x_pix, d.y_pix, d.x_img, d.y_img, d.eps = 2, 64, 8, 100, 64, 64, 6400, 6400, 1e-3
+    d.N, d.C, d.groups, d.pixels, d.x_pix, d.y_pix, d.x_img, d.y_img, d.eps = 2, 64, 8, 3000, 64, 64, 192000, 192000, 1e-3
     d.workspace_bytes = 1 << 20
     for k, v in kw.items():
         setattr(d, k, v)
@@ -33,9 +33,9 @@ def bwd(**kw):
     d = L.GroupNormBwdDesc()
     for i, f in enumerate(("x", "dy", "dx", "mean", "rstd", "scale", "shift", "workspace")):
         setattr(d, f, A + (i << 24))
-    d.N, d.C, d.groups, d.pixels = 2, 64, 8, 100
+    d.N, d.C, d.groups, d.pixels = 2, 64, 8, 3000
     d.x_pix = d.dy_pix = d.dx_pix = 64
-    d.x_img = d.dy_img = d.dx_img = 6400
+    d.x_img = d.dy_img = d.dx_img = 192000
     d.workspace_bytes = 1 << 20
     for k, v in kw.items():
         setattr(d, k, v)
@@ -57,10 +57,10 @@ COMMON = [dict(dtype=2), dict(fmt=2), dict(act=L.ACT_SOFTMAX), dict(act=9), dict
 
 @pytest.mark.parametrize("bad", COMMON + [
     dict(groups=0), dict(groups=7), dict(groups=-1), dict(x=None), dict(y=None), dict(x=A + 8), dict(y=A + 2), dict(x_pix=56),
-    dict(x_pix=68), dict(y_pix=0), dict(x_img=6336), dict(x_img=6404), dict(y_img=0), dict(mean=None), dict(rstd=None),
+    dict(x_pix=68), dict(y_pix=0), dict(x_img=191936), dict(x_img=192004), dict(y_img=0), dict(mean=None), dict(rstd=None),
     dict(scale=None), dict(shift=A + 4), dict(eps=-1.0), dict(eps=float("nan")), dict(codes=A), dict(code_scales=A),
     dict(codes=A + 4, code_scales=A), dict(codes=A, code_scales=A + 1), dict(workspace=None), dict(workspace=A + 8),
-    dict(workspace_bytes=100), dict(y=A + 128), dict(y=A + 6400), dict(y=A, y_pix=72, y_img=7200),
+    dict(workspace_bytes=100), dict(y=A + 128), dict(y=A + 6400), dict(y=A, y_pix=72, y_img=216000),
 ], ids=str)
 def test_group_norm_forward(bad):
     assert lib().miseg_group_norm_act_fwd(C.byref(fwd(**bad)), None) == L.E_INVALID_ARG
@@ -100,11 +100,13 @@ def test_null_descriptors_and_workspace_sizes():
     l = lib()
     for f in (l.miseg_group_norm_act_fwd, l.miseg_group_norm_act_bwd, l.miseg_checkpoint8_write, l.miseg_checkpoint8_read):
         assert f(None, None) == L.E_INVALID_ARG
-    for bad in ((0, 1, 8), (65536, 1, 8), (1, 0, 8), (1, 1 << 29, 8), (1, 1, 0), (1, 1, 12), (1, 1, 65544)):
-        assert l.miseg_group_norm_workspace(*bad, 0) == L.E_INVALID_ARG
-    assert 0 < l.miseg_group_norm_workspace(1, 1, 8, 0) < l.miseg_group_norm_workspace(1, 1, 8, 1) < 1 << 20
+    for bad in ((0, 1, 8, 1, 0), (65536, 1, 8, 1, 0), (1, 0, 8, 1, 0), (1, 1 << 29, 8, 1, 0), (1, 1, 0, 1, 0),
+                (1, 1, 12, 1, 0), (1, 1, 65544, 1, 0), (1, 1, 8, 0, 0), (1, 1, 8, 3, 0), (1, 1, 8, 1, 2)):
+        assert l.miseg_group_norm_workspace(*bad, 0, 0) == L.E_INVALID_ARG
+    assert l.miseg_group_norm_workspace(1, 1, 8, 1, 0, 0, 0) == 0
+    big = [l.miseg_group_norm_workspace(4, 960 * 1280, 64, 16, 0, *k) for k in ((0, 0), (1, 0), (0, 1))]
     # of the order of the statistics, never of the tensor: 4 images at 960 x 1280 with 64 channels are 629 MB
-    assert l.miseg_group_norm_workspace(4, 960 * 1280, 64, 1) < 4 << 20
+    assert 0 < big[0] < big[1] < big[2] < 4 << 20
 
 
 def test_python_refuses():
