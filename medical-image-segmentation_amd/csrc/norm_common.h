@@ -153,6 +153,11 @@ __device__ __forceinline__ void load_coef(float (&f)[8], const float* p) {
   f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
 }
 
+__device__ __forceinline__ void store_coef(float* p, const float (&f)[8]) {
+  *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
+  *reinterpret_cast<float4*>(p + 4) = make_float4(f[4], f[5], f[6], f[7]);
+}
+
 // ---- the 8-bit block format: 32 consecutive channels of a pixel share a bf16 scale, bf16(amax / 127).
 // code = rint(v / scale): |code| <= 127 because the scale's rounding moves amax / scale by at most 2^-9 of 127, less than
 // half a step.  Below 2^-119 the scale would be a subnormal number and its reciprocal infinite: such a block is zero.  A

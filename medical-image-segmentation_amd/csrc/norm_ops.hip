@@ -143,6 +143,109 @@ __global__ __launch_bounds__(kNormThreads) void gn_finalize_kernel(const float2*
   }
 }
 
+// Threads in segments of `lanes`, a power of two up to 64 or a multiple of 64: the sums over a segment, in its first thread.
+// Every thread of the block calls; `waves` holds one entry per wave.
+struct Segments {
+  int lanes, seg, t;
+  __device__ __forceinline__ Segments(int threads, int segments) {
+    const int most = threads / segments;
+    lanes = most >= 64 ? most & ~63 : 1 << (31 - __clz(most));
+    seg = threadIdx.x / lanes;
+    t = threadIdx.x - seg * lanes;
+  }
+  __device__ __forceinline__ double2 sum(double2 v, double2* waves) const {
+    for (int o = lanes < 64 ? lanes >> 1 : 32; o > 0; o >>= 1) {
+      v.x += __shfl_xor(v.x, o, 64);
+      v.y += __shfl_xor(v.y, o, 64);
+    }
+    if (lanes > 64) {
+      const int wave = threadIdx.x >> 6;
+      if ((threadIdx.x & 63) == 0) waves[wave] = v;
+      __syncthreads();
+      if (t == 0)
+        for (int i = 1; i < lanes >> 6; ++i) {
+          v.x += waves[wave + i].x;
+          v.y += waves[wave + i].y;
+        }
+    }
+    return v;
+  }
+};
+
+// The groups of a thread's 8 channels, the first of them `first` (a multiple of 8 in the slab).
+struct GroupWalk {
+  int g, left, width;
+  __device__ __forceinline__ GroupWalk(int first, int w) : width(w) {
+    g = first / w;
+    left = w - (first - g * w);
+  }
+  __device__ __forceinline__ void next() {
+    if (--left == 0) {
+      left = width;
+      ++g;
+    }
+  }
+};
+
+// Second halves of a reduction inside the pass that needs its result, where an image has few partial sums: every block adds
+// them up for itself, which saves a launch (5 us).  All channels are in one slab (C <= 512).
+// Per channel the sums over `blocks` of f(partial, block) as chan[c]; 256 threads.
+template <typename F>
+__device__ __forceinline__ void channel_sums(double2* chan, double2* tree, int blocks, int C, F f) {
+  const int wide = C < kNormThreads ? C : kNormThreads, parts = kNormThreads / wide;
+  const int i = threadIdx.x % wide, share = threadIdx.x / wide;
+  for (int c0 = 0; c0 < C; c0 += wide) {
+    const int c = c0 + i;
+    double2 sum = make_double2(0, 0);
+    if (share < parts && c < C) {
+#pragma unroll 4
+      for (int k = share; k < blocks; k += parts) {
+        const double2 v = f(k, c);
+        sum.x += v.x;
+        sum.y += v.y;
+      }
+    }
+    tree[threadIdx.x] = sum;
+    __syncthreads();
+    for (int left = parts; left > 1;) {
+      const int half = (left + 1) >> 1;
+      if (share + half < left) {
+        tree[threadIdx.x].x += tree[threadIdx.x + half * wide].x;
+        tree[threadIdx.x].y += tree[threadIdx.x + half * wide].y;
+      }
+      __syncthreads();
+      left = half;
+    }
+    if (share == 0 && c < C) chan[c] = tree[threadIdx.x];
+    __syncthreads();
+  }
+}
+// group[g] = sum over its channels of chan
+__device__ __forceinline__ void group_sums(double2* group, const double2* chan, double2* waves, int groups, int width) {
+  if (width <= 16) {
+    for (int g = threadIdx.x; g < groups; g += kNormThreads) {
+      double2 sum = chan[g * width];
+      for (int e = 1; e < width; ++e) {
+        sum.x += chan[g * width + e].x;
+        sum.y += chan[g * width + e].y;
+      }
+      group[g] = sum;
+    }
+  } else {
+    const Segments sg(kNormThreads, groups);
+    double2 sum = make_double2(0, 0);
+    if (sg.seg < groups)
+      for (int e = sg.t; e < width; e += sg.lanes) {
+        sum.x += chan[sg.seg * width + e].x;
+        sum.y += chan[sg.seg * width + e].y;
+      }
+    sum = sg.sum(sum, waves);
+    if (sg.seg < groups && sg.t == 0) group[sg.seg] = sum;
+  }
+  __syncthreads();
+}
+constexpr int kFewChannels = 512;
+
 // ---------------------------------------------------------------------------- one pass: activated result, checkpoint
 // y = act(x a + b) and the checkpoint of x s + t (of x without s), either or both.  Coefficients per channel, `cimg` from
 // one image's to the next's.  A block makes one sweep of U pixels per thread where there is work for 32768 blocks: short
@@ -158,15 +261,67 @@ struct PassArgs {
   long long xps, ximg, yps, yimg, cimg;
   int pixels, C;
   NormGrid g;
+  // FIN: group normalisation out of the partial statistics
+  const float2* part;
+  int part_blocks, part_chunk, groups;
+  const float *gamma, *beta;
+  float *mean, *rstd, *scale, *shift;
+  float eps;
 };
 
-template <typename T, int ACT, bool Y, bool Q>
+// The statistics of the groups of image n out of the blocks' as (mean, rstd) in group[], and those of block 0 to memory.
+__device__ __forceinline__ void pass_statistics(const PassArgs& p, int n, double2* group) {
+  __shared__ double2 chan[kFewChannels], tree[kNormThreads], waves[kNormThreads / 64];
+  const float2* part = p.part + (long long)n * p.part_blocks * p.C;
+  const int last = p.pixels - (p.part_blocks - 1) * p.part_chunk, width = p.C / p.groups;
+  channel_sums(chan, tree, p.part_blocks, p.C, [&](int k, int c) {
+    const float2 v = part[k * p.C + c];
+    const double count = k == p.part_blocks - 1 ? last : p.part_chunk, m = v.x;
+    return make_double2(count * m, (double)v.y + count * m * m);
+  });
+  group_sums(group, chan, waves, p.groups, width);
+  const double rcount = 1.0 / ((double)p.pixels * width);
+  for (int g = threadIdx.x; g < p.groups; g += kNormThreads) {
+    const double m = group[g].x * rcount;
+    double var = group[g].y * rcount - m * m;
+    if (var < 0) var = 0;
+    const double rs = 1.0 / sqrt(var + (double)p.eps);
+    group[g] = make_double2(m, rs);
+    if (blockIdx.x == 0) {
+      p.mean[n * p.groups + g] = (float)m;
+      p.rstd[n * p.groups + g] = (float)rs;
+    }
+  }
+  __syncthreads();
+}
+
+template <typename T, int ACT, bool Y, bool Q, bool FIN>
 __global__ __launch_bounds__(kNormThreads) void norm_pass_kernel(PassArgs p) {
   constexpr int ES = Elem<T>::bytes, U = 4;
   NormWalk w(p.g, gridDim.x - 1 - blockIdx.x, p.pixels, p.C);
-  if (w.r >= p.g.rows) return;                    // lanes past the last channel stay for the exchange in quantise8
   float a[8], b[8], s[8], t[8];
-  if (w.active) {
+  if constexpr (FIN) {
+    __shared__ double2 group[kFewChannels];
+    pass_statistics(p, w.n, group);
+    if (w.active) {
+      GroupWalk gw(w.c, p.C / p.groups);
+#pragma unroll
+      for (int j = 0; j < 8; ++j, gw.next()) {
+        const double2 q = group[gw.g];
+        const double sc = p.gamma ? p.gamma[w.c + j] * q.y : q.y;
+        a[j] = (float)sc;
+        b[j] = (float)((p.beta ? p.beta[w.c + j] : 0.0) - q.x * sc);
+        s[j] = (float)q.y;
+        t[j] = (float)(-q.x * q.y);
+      }
+      if (blockIdx.x == 0 && w.r == 0) {
+        store_coef(p.scale + (long long)w.n * p.C + w.c, a);
+        store_coef(p.shift + (long long)w.n * p.C + w.c, b);
+      }
+    }
+  }
+  if (w.r >= p.g.rows) return;                    // lanes past the last channel stay for the exchange in quantise8
+  if (!FIN && w.active) {
     if (Y) { load_coef(a, p.a + w.n * p.cimg + w.c); load_coef(b, p.b + w.n * p.cimg + w.c); }
     if (Q && p.s) { load_coef(s, p.s + w.n * p.cimg + w.c); load_coef(t, p.t + w.n * p.cimg + w.c); }
   }
@@ -195,7 +350,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_pass_kernel(PassArgs p) {
       }
       if constexpr (Q) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] = !w.active ? 0.f : p.s ? fmaf(f[j], s[j], t[j]) : f[j];
+        for (int j = 0; j < 8; ++j) o[j] = !w.active ? 0.f : FIN || p.s ? fmaf(f[j], s[j], t[j]) : f[j];
         const Quant8 q = quantise8(o);
         if (w.active) {
           *reinterpret_cast<uint2*>(cp + u * cstep) = q.codes;
@@ -276,6 +431,8 @@ struct BwdArgs {
   long long xps, ximg, dps, dimg, ops, oimg;
   int pixels, C, groups, images;
   NormGrid g;
+  const float2* part;                              // FIN: the blocks' sums, `part_blocks` an image
+  int part_blocks;
 };
 
 template <typename T, bool CK> struct BwdLoad {
@@ -493,32 +650,36 @@ __device__ __forceinline__ void gn_bwd_params(const double2* sums, int images, i
   if (dgamma) dgamma[c] = (float)b;
 }
 
-// Second pass: dx = a g + (x - cm) cp + cq.  With `sums`, the blocks past the last pixels add up the parameters' gradients.
-template <typename T, int ACT, bool CK>
-__global__ __launch_bounds__(kNormThreads) void gn_bwd_apply_kernel(BwdArgs p) {
-  constexpr int ES = Elem<T>::bytes, U = 4;
-  if ((int)blockIdx.x == p.g.blocks) {
-    if (blockIdx.z == 0)
-      for (int i = threadIdx.x; i < p.g.cw * 8; i += kNormThreads)
-        if (const int c = blockIdx.y * p.g.cw * 8 + i; c < p.C) gn_bwd_params(p.sums, p.images, p.C, c, p.dgamma, p.dbeta);
-    return;
-  }
-  NormWalk w(p.g, p.g.blocks - 1 - blockIdx.x, p.pixels, p.C);
-  if (!w.active) return;
-  float za[8], zb[8], a[8], m[8], kp[8], kq[8];
-  const long long cat = (long long)w.n * p.C + w.c;
-  load_coef(a, p.a + cat);
+template <bool CK>
+__device__ __forceinline__ void group_bwd_coef(float (&za)[8], float (&zb)[8], float (&m)[8], float (&rs)[8], const BwdArgs& p,
+                                               int n, int c, int width) {
+  const long long at = (long long)n * p.C + c;
   if constexpr (CK) {
-    load_coef(za, p.cm + cat);
-    load_coef(zb, p.cz + cat);
-  } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) za[j] = a[j];
-    load_coef(zb, p.b + cat);
-    load_coef(m, p.cm + cat);
+    for (int j = 0; j < 8; ++j) {
+      za[j] = p.gamma ? p.gamma[c + j] : 1.f;
+      zb[j] = p.beta ? p.beta[c + j] : 0.f;
+      m[j] = 0.f;
+      rs[j] = 1.f;
+    }
+  } else {
+    load_coef(za, p.a + at);
+    load_coef(zb, p.b + at);
+    GroupWalk gw(c, width);
+    gw.g += n * p.groups;
+#pragma unroll
+    for (int j = 0; j < 8; ++j, gw.next()) {
+      m[j] = p.mean[gw.g];
+      rs[j] = p.rstd[gw.g];
+    }
   }
-  load_coef(kp, p.cp + cat);
-  load_coef(kq, p.cq + cat);
+}
+
+template <typename T, int ACT, bool CK>
+__device__ __forceinline__ void bwd_apply(const BwdArgs& p, const NormWalk& w, const float (&a)[8], const float (&za)[8],
+                                          const float (&zb)[8], const float (&m)[8], const float (&kp)[8],
+                                          const float (&kq)[8]) {
+  constexpr int ES = Elem<T>::bytes, U = 4;
   BwdFrom<T, CK> from(p, w);
   const int rows = p.g.rows;
   int px = w.p0 + w.r;
@@ -546,6 +707,74 @@ __global__ __launch_bounds__(kNormThreads) void gn_bwd_apply_kernel(BwdArgs p) {
   }
 }
 
+// Second pass: dx = a g + (x - cm) cp + cq.  With dgamma or dbeta due, the blocks past the last pixels add them up.
+// FIN: the groups' sums out of the blocks'.
+template <typename T, int ACT, bool CK, bool FIN>
+__global__ __launch_bounds__(kNormThreads) void gn_bwd_apply_kernel(BwdArgs p) {
+  if constexpr (FIN) {
+    __shared__ double2 chan[kFewChannels], group[kFewChannels], tree[kNormThreads], waves[kNormThreads / 64];
+    const bool params = (int)blockIdx.x == p.g.blocks;
+    if (params && blockIdx.z != 0) return;
+    const int n = blockIdx.z;
+    const float2* part = p.part + (long long)n * p.part_blocks * p.C;
+    channel_sums(chan, tree, params ? p.images * p.part_blocks : p.part_blocks, p.C, [&](int k, int c) {
+      const float2 v = part[k * p.C + c];
+      const double sc = params ? 1.0 : (double)p.a[(long long)n * p.C + c];
+      return make_double2(sc * v.x, sc * v.y);
+    });
+    if (params) {
+      for (int c = threadIdx.x; c < p.C; c += kNormThreads) {
+        if (p.dbeta) p.dbeta[c] = (float)chan[c].x;
+        if (p.dgamma) p.dgamma[c] = (float)chan[c].y;
+      }
+      return;
+    }
+    const int width = p.C / p.groups;
+    group_sums(group, chan, waves, p.groups, width);
+    NormWalk w(p.g, p.g.blocks - 1 - blockIdx.x, p.pixels, p.C);
+    if (!w.active) return;
+    float za[8], zb[8], a[8], m[8], kp[8], kq[8];
+    group_bwd_coef<CK>(za, zb, m, kp, p, n, w.c, width);
+    if constexpr (CK) load_coef(a, p.a + (long long)n * p.C + w.c);
+    else
+#pragma unroll
+      for (int j = 0; j < 8; ++j) a[j] = za[j];
+    const double rcount = 1.0 / ((double)p.pixels * width);
+    GroupWalk gw(w.c, width);
+#pragma unroll
+    for (int j = 0; j < 8; ++j, gw.next()) {
+      const double2 k = group[gw.g];
+      kp[j] = (float)(-k.y * rcount * kp[j]);
+      kq[j] = (float)(-k.x * rcount);
+    }
+    bwd_apply<T, ACT, CK>(p, w, a, za, zb, m, kp, kq);
+  } else {
+    if ((int)blockIdx.x == p.g.blocks) {
+      if (blockIdx.z == 0)
+        for (int i = threadIdx.x; i < p.g.cw * 8; i += kNormThreads)
+          if (const int c = blockIdx.y * p.g.cw * 8 + i; c < p.C) gn_bwd_params(p.sums, p.images, p.C, c, p.dgamma, p.dbeta);
+      return;
+    }
+    NormWalk w(p.g, p.g.blocks - 1 - blockIdx.x, p.pixels, p.C);
+    if (!w.active) return;
+    float za[8], zb[8], a[8], m[8], kp[8], kq[8];
+    const long long cat = (long long)w.n * p.C + w.c;
+    load_coef(a, p.a + cat);
+    if constexpr (CK) {
+      load_coef(za, p.cm + cat);
+      load_coef(zb, p.cz + cat);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) za[j] = a[j];
+      load_coef(zb, p.b + cat);
+      load_coef(m, p.cm + cat);
+    }
+    load_coef(kp, p.cp + cat);
+    load_coef(kq, p.cq + cat);
+    bwd_apply<T, ACT, CK>(p, w, a, za, zb, m, kp, kq);
+  }
+}
+
 // ------------------------------------------------------------------------------------------------ small maps
 // A block takes all pixels of some groups of one image and keeps them in registers between the statistics and the result:
 // one launch, x read once.  A thread holds up to V pixels of its 8 channels.
@@ -561,50 +790,6 @@ __device__ __forceinline__ int small_block(int blocks) {
   const int per = blocks >> 3, b = blockIdx.x;
   return b < per * 8 ? (b & 7) * per + (b >> 3) : b;
 }
-
-// Threads in segments of `lanes`, a power of two up to 64 or a multiple of 64: the sums over a segment, in its first thread.
-// Every thread of the block calls; `waves` holds one entry per wave.
-struct Segments {
-  int lanes, seg, t;
-  __device__ __forceinline__ Segments(int threads, int segments) {
-    const int most = threads / segments;
-    lanes = most >= 64 ? most & ~63 : 1 << (31 - __clz(most));
-    seg = threadIdx.x / lanes;
-    t = threadIdx.x - seg * lanes;
-  }
-  __device__ __forceinline__ double2 sum(double2 v, double2* waves) const {
-    for (int o = lanes < 64 ? lanes >> 1 : 32; o > 0; o >>= 1) {
-      v.x += __shfl_xor(v.x, o, 64);
-      v.y += __shfl_xor(v.y, o, 64);
-    }
-    if (lanes > 64) {
-      const int wave = threadIdx.x >> 6;
-      if ((threadIdx.x & 63) == 0) waves[wave] = v;
-      __syncthreads();
-      if (t == 0)
-        for (int i = 1; i < lanes >> 6; ++i) {
-          v.x += waves[wave + i].x;
-          v.y += waves[wave + i].y;
-        }
-    }
-    return v;
-  }
-};
-
-// The groups of a thread's 8 channels, the first of them `first` (a multiple of 8 in the slab).
-struct GroupWalk {
-  int g, left, width;
-  __device__ __forceinline__ GroupWalk(int first, int w) : width(w) {
-    g = first / w;
-    left = w - (first - g * w);
-  }
-  __device__ __forceinline__ void next() {
-    if (--left == 0) {
-      left = width;
-      ++g;
-    }
-  }
-};
 
 struct SmallFwdArgs {
   const char* x;
@@ -736,11 +921,8 @@ __global__ __launch_bounds__(TB) void gn_small_fwd_kernel(SmallFwdArgs p) {
       b[j] = (float)((p.beta ? p.beta[c + j] : 0.0) - q.x * sc);
     }
     if (r == 0) {
-      float4 *pa = reinterpret_cast<float4*>(p.a + (long long)n * p.C + c), *pb = reinterpret_cast<float4*>(p.b + (long long)n * p.C + c);
-      pa[0] = make_float4(a[0], a[1], a[2], a[3]);
-      pa[1] = make_float4(a[4], a[5], a[6], a[7]);
-      pb[0] = make_float4(b[0], b[1], b[2], b[3]);
-      pb[1] = make_float4(b[4], b[5], b[6], b[7]);
+      store_coef(p.a + (long long)n * p.C + c, a);
+      store_coef(p.b + (long long)n * p.C + c, b);
     }
     char* yp = p.y + (n * p.yimg + c) * ES;
     if (p.act == NA_RELU) small_fwd_finish<T, NA_RELU, V>(yp, p.yps, v, a, b, r, rows, p.pixels);
@@ -825,31 +1007,6 @@ __device__ __forceinline__ void small_bwd_finish(char* op, long long ops, const 
   }
 }
 
-template <bool CK>
-__device__ __forceinline__ void small_bwd_coef(float (&za)[8], float (&zb)[8], float (&m)[8], float (&rs)[8], const BwdArgs& p,
-                                               int n, int c, int width) {
-  const long long at = (long long)n * p.C + c;
-  if constexpr (CK) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      za[j] = p.gamma ? p.gamma[c + j] : 1.f;
-      zb[j] = p.beta ? p.beta[c + j] : 0.f;
-      m[j] = 0.f;
-      rs[j] = 1.f;
-    }
-  } else {
-    load_coef(za, p.a + at);
-    load_coef(zb, p.b + at);
-    GroupWalk gw(c, width);
-    gw.g += n * p.groups;
-#pragma unroll
-    for (int j = 0; j < 8; ++j, gw.next()) {
-      m[j] = p.mean[gw.g];
-      rs[j] = p.rstd[gw.g];
-    }
-  }
-}
-
 template <typename T, bool CK, int TB, int V>
 __global__ __launch_bounds__(TB) void gn_small_bwd_kernel(SmallBwdArgs q) {
   constexpr int ES = Elem<T>::bytes;
@@ -878,7 +1035,7 @@ __global__ __launch_bounds__(TB) void gn_small_bwd_kernel(SmallBwdArgs q) {
   }
   if (active) {
     float za[8], zb[8], m[8], rs[8], s1[8], s2[8];
-    small_bwd_coef<CK>(za, zb, m, rs, p, n, c, width);
+    group_bwd_coef<CK>(za, zb, m, rs, p, n, c, width);
 #pragma unroll
     for (int j = 0; j < 8; ++j) s1[j] = s2[j] = 0.f;
     if (q.act == NA_RELU) small_bwd_sums<T, NA_RELU, CK, V>(s1, s2, v, za, zb, m, r, rows, p.pixels);
@@ -937,7 +1094,7 @@ __global__ __launch_bounds__(TB) void gn_small_bwd_kernel(SmallBwdArgs q) {
   if (!active) return;
   const double rcount = 1.0 / ((double)p.pixels * width);
   float za[8], zb[8], m[8], a[8], kp[8], kq[8];   // read again rather than held over the exchange: registers are short
-  small_bwd_coef<CK>(za, zb, m, kp, p, n, c, width);
+  group_bwd_coef<CK>(za, zb, m, kp, p, n, c, width);
   if constexpr (CK) load_coef(a, p.a + (long long)n * p.C + c);
   else
 #pragma unroll
@@ -1043,6 +1200,20 @@ static int images_per_step(long long N, long long image_bytes) {
   return (int)(n < 1 ? 1 : n < N ? n : N);
 }
 
+// Whether an image's partial sums are few enough for every block of the second pass to add them up itself: 4096 of them
+// (32 KB), from blocks that read at most 192 KB each.
+constexpr int kFewEntries = 4096, kFewBlocks = 256, kFewPass = 1024;
+constexpr long long kFewBytes = 192 << 10;
+static bool few_partials(long long N, long long pixels, int C, int bytes, NormGrid& g) {
+  if (C > kFewChannels) return false;
+  const long long most = kFewEntries / C, spread = (kFewBlocks + N - 1) / N;
+  g = norm_grid(1, pixels, C, 1, 1);
+  const long long deep = (pixels + 4 * g.rows - 1) / (4 * g.rows);     // blocks of the four sweeps that are in flight together
+  const long long some = spread < most ? spread : most;
+  g = norm_grid(1, pixels, C, (int)(deep < some ? deep : some), 1);
+  return (long long)g.chunk * C * bytes <= kFewBytes;
+}
+
 static long long round_up(long long v) { return (v + 255) / 256 * 256; }
 
 // The blocks' partial sums, for steps of any number of images: norm_grid gives at most max(want, images x slabs) + images x
@@ -1075,10 +1246,12 @@ static void launch_pass(const PassArgs& p, int N, int storage, int act, hipStrea
   by_type_act(storage, act, [&](auto t, auto a) {
     typedef decltype(t) T;
     constexpr int A = decltype(a)::act;
-    if (p.y && p.codes) hipLaunchKernelGGL((norm_pass_kernel<T, A, true, true>), grid, dim3(kNormThreads), 0, s, p);
-    else if (p.y) hipLaunchKernelGGL((norm_pass_kernel<T, A, true, false>), grid, dim3(kNormThreads), 0, s, p);
+    if (p.part && p.codes) hipLaunchKernelGGL((norm_pass_kernel<T, A, true, true, true>), grid, dim3(kNormThreads), 0, s, p);
+    else if (p.part) hipLaunchKernelGGL((norm_pass_kernel<T, A, true, false, true>), grid, dim3(kNormThreads), 0, s, p);
+    else if (p.y && p.codes) hipLaunchKernelGGL((norm_pass_kernel<T, A, true, true, false>), grid, dim3(kNormThreads), 0, s, p);
+    else if (p.y) hipLaunchKernelGGL((norm_pass_kernel<T, A, true, false, false>), grid, dim3(kNormThreads), 0, s, p);
     else if constexpr (A == NA_NONE)
-      hipLaunchKernelGGL((norm_pass_kernel<T, NA_NONE, false, true>), grid, dim3(kNormThreads), 0, s, p);
+      hipLaunchKernelGGL((norm_pass_kernel<T, NA_NONE, false, true, false>), grid, dim3(kNormThreads), 0, s, p);
   });
 }
 
@@ -1129,6 +1302,19 @@ int launch_group_norm_fwd(const miseg_group_norm_desc* d, hipStream_t s) {
     qs = (float*)ws;
     qt = (float*)(ws + round_up(4LL * d->N * d->C));
   }
+  if (NormGrid g; few_partials(d->N, d->pixels, d->C, bytes, g)) {
+    by_type_act(storage, NA_NONE, [&](auto t, auto) {
+      hipLaunchKernelGGL((gn_stats_kernel<decltype(t)>), dim3(g.blocks, g.ny, d->N), dim3(kNormThreads), 0, s,
+                         (const char*)d->x, (long long)d->x_pix, d->x_img, (int)d->pixels, d->C, g, part);
+    });
+    PassArgs p{(const char*)d->x, (char*)d->y, (signed char*)d->codes, (bf16_t*)d->code_scales, nullptr, nullptr, nullptr,
+               nullptr, d->x_pix, d->x_img, d->y_pix, d->y_img, d->C, (int)d->pixels, d->C,
+               norm_grid(d->N, d->pixels, d->C, kFewPass, kPassLeast), part, g.blocks, g.chunk, d->groups, d->gamma, d->beta,
+               d->mean, d->rstd, d->scale, d->shift, d->eps};
+    launch_pass(p, d->N, storage, act_of(d->act), s);
+    MISEG_CHECK_HIP(hipGetLastError());
+    return MISEG_OK;
+  }
   const int step = images_per_step(d->N, d->pixels * d->C * bytes);
   for (int n0 = 0; n0 < d->N; n0 += step) {
     const int n = d->N - n0 < step ? d->N - n0 : step;
@@ -1144,7 +1330,8 @@ int launch_group_norm_fwd(const miseg_group_norm_desc* d, hipStream_t s) {
                        d->shift + cat, qs, qt);
     PassArgs p{x, (char*)d->y + n0 * d->y_img * bytes, (signed char*)d->codes, (bf16_t*)d->code_scales, d->scale + cat,
                d->shift + cat, qs, qt, d->x_pix, d->x_img, d->y_pix, d->y_img, d->C, (int)d->pixels, d->C,
-               norm_grid(n, d->pixels, d->C, kPassBlocks, kPassLeast)};
+               norm_grid(n, d->pixels, d->C, kPassBlocks, kPassLeast), nullptr, 0, 0, 0, nullptr, nullptr, nullptr, nullptr,
+               nullptr, nullptr, 0.f};
     if (p.codes) {
       p.codes += n0 * d->pixels * d->C;
       p.scales += n0 * d->pixels * ((d->C + 31) / 32);
@@ -1210,10 +1397,12 @@ int launch_group_norm_bwd(const miseg_group_norm_bwd_desc* d, hipStream_t s) {
   ws += gn_partials(d->N, d->pixels, d->C);
   const long long coef = round_up(4LL * d->N * d->C);
   float *cm = (float*)ws, *cz = (float*)(ws + coef), *cp = (float*)(ws + 2 * coef), *cq = (float*)(ws + 3 * coef);
+  NormGrid few;
+  const bool fin = few_partials(d->N, d->pixels, d->C, bytes, few);
   const long long dbytes = d->pixels * d->C * bytes, xbytes = ck ? d->pixels * (d->C + 2 * ((d->C + 31) / 32)) : dbytes;
   // both stay in the cache if they can; else dy alone; else the last pixels of both
   const bool alone = xbytes + dbytes > kCacheBytes && dbytes <= kCacheBytes;
-  const int step = images_per_step(d->N, alone ? dbytes : xbytes + dbytes);
+  const int step = fin ? d->N : images_per_step(d->N, alone ? dbytes : xbytes + dbytes);
   for (int n0 = 0; n0 < d->N; n0 += step) {
     const int n = d->N - n0 < step ? d->N - n0 : step;
     const long long cat = (long long)n0 * d->C, gat = (long long)n0 * d->groups;
@@ -1221,7 +1410,7 @@ int launch_group_norm_bwd(const miseg_group_norm_bwd_desc* d, hipStream_t s) {
               (char*)d->dx + n0 * d->dx_img * bytes, (const signed char*)d->codes, (const bf16_t*)d->code_scales,
               d->mean + gat, d->rstd + gat, d->scale + cat, d->shift + cat, d->gamma, d->beta, cm, cz, cp, cq, nullptr,
               d->dgamma, d->dbeta, d->x_pix, d->x_img, d->dy_pix, d->dy_img, d->dx_pix, d->dx_img, (int)d->pixels, d->C,
-              d->groups, d->N, norm_grid(n, d->pixels, d->C, kStatBlocks, kStatLeast)};
+              d->groups, d->N, fin ? few : norm_grid(n, d->pixels, d->C, kStatBlocks, kStatLeast), part, few.blocks};
     if (ck) {
       p.codes += n0 * d->pixels * d->C;
       p.scales += n0 * d->pixels * ((d->C + 31) / 32);
@@ -1236,17 +1425,20 @@ int launch_group_norm_bwd(const miseg_group_norm_bwd_desc* d, hipStream_t s) {
       else if (alone) hipLaunchKernelGGL((gn_bwd_reduce_kernel<T, A, false, true>), grid, dim3(kNormThreads), 0, s, p, part);
       else hipLaunchKernelGGL((gn_bwd_reduce_kernel<T, A, false, false>), grid, dim3(kNormThreads), 0, s, p, part);
     });
-    hipLaunchKernelGGL(gn_bwd_finalize_kernel, dim3(d->groups, n), dim3(kNormThreads), 0, s, p, part, blocks, ck ? 1 : 0,
-                       sums + cat, cm, cz, cp, cq);
-    p.g = norm_grid(n, d->pixels, d->C, kPassBlocks, kPassLeast);
+    if (!fin)
+      hipLaunchKernelGGL(gn_bwd_finalize_kernel, dim3(d->groups, n), dim3(kNormThreads), 0, s, p, part, blocks, ck ? 1 : 0,
+                         sums + cat, cm, cz, cp, cq);
+    p.g = norm_grid(n, d->pixels, d->C, fin ? kFewPass : kPassBlocks, kPassLeast);
     const bool params = n0 + n == d->N && (d->dgamma || d->dbeta);
     if (params) p.sums = sums;
     by_type_act(storage, act, [&](auto t, auto a) {
       typedef decltype(t) T;
       constexpr int A = decltype(a)::act;
       const dim3 grid(p.g.blocks + (params ? 1 : 0), p.g.ny, n);
-      if (ck) hipLaunchKernelGGL((gn_bwd_apply_kernel<T, A, true>), grid, dim3(kNormThreads), 0, s, p);
-      else hipLaunchKernelGGL((gn_bwd_apply_kernel<T, A, false>), grid, dim3(kNormThreads), 0, s, p);
+      if (ck && fin) hipLaunchKernelGGL((gn_bwd_apply_kernel<T, A, true, true>), grid, dim3(kNormThreads), 0, s, p);
+      else if (ck) hipLaunchKernelGGL((gn_bwd_apply_kernel<T, A, true, false>), grid, dim3(kNormThreads), 0, s, p);
+      else if (fin) hipLaunchKernelGGL((gn_bwd_apply_kernel<T, A, false, true>), grid, dim3(kNormThreads), 0, s, p);
+      else hipLaunchKernelGGL((gn_bwd_apply_kernel<T, A, false, false>), grid, dim3(kNormThreads), 0, s, p);
     });
   }
   MISEG_CHECK_HIP(hipGetLastError());
@@ -1270,7 +1462,8 @@ int launch_checkpoint8_write(const miseg_checkpoint8_desc* d, hipStream_t s) {
                   "checkpoint8_write: y must be a view like x, and be x, another channel range of its buffer or apart from it");
   PassArgs p{(const char*)d->x, (char*)d->y, (signed char*)d->codes, (bf16_t*)d->code_scales, d->y_a, d->y_b, d->code_a,
              d->code_b, d->x_pix, d->x_img, d->y_pix, d->y_img, d->coef_img, (int)d->pixels, d->C,
-             norm_grid(d->N, d->pixels, d->C, kPassBlocks, kPassLeast)};
+             norm_grid(d->N, d->pixels, d->C, kPassBlocks, kPassLeast), nullptr, 0, 0, 0, nullptr, nullptr, nullptr, nullptr,
+             nullptr, nullptr, 0.f};
   launch_pass(p, d->N, storage_of(d->dtype, d->fmt), act_of(d->act), s);
   MISEG_CHECK_HIP(hipGetLastError());
   return MISEG_OK;

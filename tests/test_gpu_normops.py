@@ -194,6 +194,33 @@ def test_checkpoint_of_the_forward_pass_and_backward_out_of_it(ops, shape, dt):
         close(dbeta, wb, tb)
 
 
+# one image in a launch of its own, several; both tensors of the backward pass in the memory-side cache, one of them, none
+@pytest.mark.parametrize("shape", [(5, 480, 640, 64, 16), (3, 960, 1280, 48, 12), (1, 1920, 1280, 48, 6), (2, 300, 400, 1032, 43)], ids=str)
+@pytest.mark.parametrize("checkpoint", [False, True])
+def test_large_maps(ops, shape, checkpoint):
+    n, h, w, c, groups = shape
+    dt, act = torch.bfloat16, "relu"
+    x, dy, gamma, beta = make(n, h, w, c, dt, seed=1)
+    y, saved = ops.group_norm_act(x, gamma, beta, groups, act=act, checkpoint=checkpoint)
+    dx, dgamma, dbeta = ops.group_norm_act_backward(dy, saved)
+    sums = torch.zeros(4, c, dtype=torch.float64, device="cuda")
+    for i in range(n):                                          # an image at a time: the references are in 64 bits
+        one = slice(i, i + 1)
+        part = ops.Saved(None, None, saved.mean[one], saved.rstd[one], saved.scale[one], saved.shift[one], gamma, beta, groups, act)
+        check_forward(x[one], y[one], part, gamma, beta, groups, 1e-3, act)
+        if checkpoint:
+            xhat = values(ops.Checkpoint8(saved.checkpoint.codes[one], saved.checkpoint.scales[one]))
+            z = xhat * gamma.double() + beta.double()
+        else:
+            xhat = (x[one].double() - spread(part.mean.double(), c)) * spread(part.rstd.double(), c)
+            z = x[one].double() * part.scale.double()[:, None, None] + part.shift.double()[:, None, None]
+        wdx, wg, wb, tx, tg, tb = backward64(xhat, z, None, dy[one], part.scale.double(), groups, act, dt)
+        close(dx[one], wdx, tx)
+        sums += torch.stack([wg, wb, tg, tb])
+    close(dgamma, sums[0], sums[2])
+    close(dbeta, sums[1], sums[3])
+
+
 def test_parameters_may_be_missing(ops):
     x, dy, gamma, beta = make(2, 9, 11, 48, torch.bfloat16)
     ones, zeros = torch.ones_like(gamma), torch.zeros_like(beta)
