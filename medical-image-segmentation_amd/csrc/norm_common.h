@@ -92,7 +92,7 @@ template <typename T> __device__ __forceinline__ Vec8<T> pack8(const float (&f)[
 enum { NA_NONE = 0, NA_RELU = 1, NA_SILU = 2 };
 __device__ __forceinline__ float sigmoid_f32(float z) { return __builtin_amdgcn_rcpf(1.f + __expf(-z)); }
 template <int ACT> __device__ __forceinline__ float act_fwd(float z) {
-  if constexpr (ACT == NA_RELU) return z < 0.f ? 0.f : z;            // a NaN stays one
+  if constexpr (ACT == NA_RELU) return __builtin_elementwise_maximum(z, 0.f);   // a NaN stays one
   if constexpr (ACT == NA_SILU) return z * sigmoid_f32(z);
   return z;
 }
@@ -153,6 +153,15 @@ __device__ __forceinline__ void load_coef(float (&f)[8], const float* p) {
   f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
 }
 
+// Parameters of 8 channels, `none` where there are none; a slice of a flat parameter buffer need not be aligned.
+__device__ __forceinline__ void load_param(float (&f)[8], const float* p, int c, float none) {
+  if (p && ((uintptr_t)p & 15) == 0) {
+    load_coef(f, p + c);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = p ? p[c + j] : none;
+  }
+}
 __device__ __forceinline__ void store_coef(float* p, const float (&f)[8]) {
   *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
   *reinterpret_cast<float4*>(p + 4) = make_float4(f[4], f[5], f[6], f[7]);

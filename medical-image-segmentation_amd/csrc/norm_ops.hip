@@ -4,145 +4,11 @@
 
 namespace miseg {
 
-// ------------------------------------------------------------------------------------------------ forward statistics
-// Per block and channel: mean and sum of squared differences from it.  A thread sums (x - k) and (x - k)^2 with k its own
-// first value, so that an offset of the channel that is large against its spread does not cancel; threads and blocks are
-// joined by counts, means and sums of squares.
-template <typename T>
-__global__ __launch_bounds__(kNormThreads) void gn_stats_kernel(const char* x, long long xps, long long ximg, int pixels,
-                                                                int C, NormGrid g, float2* __restrict__ part) {
-  constexpr int ES = Elem<T>::bytes, U = 4;
-  __shared__ float lmean[kNormThreads * 8], lm2[kNormThreads * 8];
-  __shared__ int lcount[kNormThreads];
-  __shared__ double2 lsum[kNormThreads];
-  NormWalk w(g, blockIdx.x, pixels, C);
-  float k[8], s1[8], s2[8];
-  int count = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) k[j] = s1[j] = s2[j] = 0.f;
-  int px = w.p0 + w.r;
-  if (w.active && px < w.p1) {
-    const char* xp = x + (w.n * ximg + px * xps + w.c) * ES;
-    const long long step = g.rows * xps * ES;
-    unpack8(k, load8<T>(xp));
-    for (; px < w.p1; px += U * g.rows, xp += U * step) {
-      Vec8<T> v[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (px + u * g.rows < w.p1) v[u] = load8<T>(xp + u * step);
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (px + u * g.rows < w.p1) {
-          float f[8];
-          unpack8(f, v[u]);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float d = f[j] - k[j];
-            s1[j] += d;
-            s2[j] = fmaf(d, d, s2[j]);
-          }
-          ++count;
-        }
-    }
-  }
-  const float rc = count ? 1.f / (float)count : 0.f;
-  if ((int)threadIdx.x == w.r * g.cw) lcount[w.r] = count;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    lmean[threadIdx.x * 8 + j] = k[j] + s1[j] * rc;
-    lm2[threadIdx.x * 8 + j] = s2[j] - s1[j] * s1[j] * rc;
-  }
-  __syncthreads();
-  // channel i of the slab from `parts` threads, then from one
-  const int wide = g.cw * 8, parts = wide < kNormThreads ? kNormThreads / wide : 1;
-  for (int i0 = 0; i0 < wide; i0 += kNormThreads) {
-    const int i = i0 + (int)threadIdx.x % wide, q = (int)threadIdx.x / wide;
-    double sum = 0, sq = 0;
-    if (q < parts && i < wide)
-      for (int r = q; r < g.rows; r += parts) {
-        const double m = lmean[r * wide + i], n = lcount[r];
-        sum += n * m;
-        sq += lm2[r * wide + i] + n * m * m;
-      }
-    if (parts > 1) {
-      lsum[threadIdx.x] = make_double2(sum, sq);
-      __syncthreads();
-      if (q == 0)
-        for (int t = 1; t < parts; ++t) {
-          sum += lsum[t * wide + i].x;
-          sq += lsum[t * wide + i].y;
-        }
-    }
-    const int c = blockIdx.y * wide + i;
-    if (q == 0 && i < wide && c < C) {
-      const double mean = sum / (w.p1 - w.p0);
-      part[((long long)w.n * gridDim.x + blockIdx.x) * C + c] = make_float2((float)mean, (float)(sq - sum * mean));
-    }
-  }
-}
+// Sweeps whose pixels are all there go without a check per load.
+struct WholeTag { constexpr operator bool() const { return true; } };
+struct PartTag { constexpr operator bool() const { return false; } };
 
-// Sum over the 256 threads of a block, in every thread.
-__device__ __forceinline__ double block_sum(double v, double* lds) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-  __syncthreads();
-  return lds[0] + lds[1] + lds[2] + lds[3];
-}
-
-// One block per (group, image): the blocks' statistics of the group's channels in 64 bits, then the coefficients.
-__global__ __launch_bounds__(kNormThreads) void gn_finalize_kernel(const float2* __restrict__ part, int blocks, int chunk,
-                                                                   long long pixels, int C, int groups,
-                                                                   const float* __restrict__ gamma,
-                                                                   const float* __restrict__ beta, float eps,
-                                                                   float* __restrict__ mean, float* __restrict__ rstd,
-                                                                   float* __restrict__ scale, float* __restrict__ shift,
-                                                                   float* __restrict__ qs, float* __restrict__ qt) {
-  __shared__ double lds[4];
-  const int w = C / groups, g = blockIdx.x, n = blockIdx.y;
-  double s = 0, q = 0;
-  const int entries = blocks * w, last = (int)(pixels - (long long)(blocks - 1) * chunk);
-  const float2* pp = part + (long long)n * blocks * C + g * w;
-  constexpr int U = 8;                             // loads in flight: the kernel waits for nothing else
-  for (int e0 = threadIdx.x; e0 < entries; e0 += U * kNormThreads) {
-    float2 v[U];
-    int count[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int e = e0 + u * kNormThreads, b = e / w;
-      count[u] = e >= entries ? 0 : b == blocks - 1 ? last : chunk;
-      v[u] = e < entries ? pp[(long long)b * C + (e - b * w)] : make_float2(0.f, 0.f);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const double n = count[u], m = v[u].x;
-      s += n * m;
-      q += (double)v[u].y + n * m * m;
-    }
-  }
-  s = block_sum(s, lds);
-  q = block_sum(q, lds);
-  const double count = (double)pixels * w, m = s / count;
-  double var = q / count - m * m;
-  if (var < 0) var = 0;
-  const double r = 1.0 / sqrt(var + (double)eps);
-  if (threadIdx.x == 0) {
-    mean[n * groups + g] = (float)m;
-    rstd[n * groups + g] = (float)r;
-  }
-  for (int i = threadIdx.x; i < w; i += kNormThreads) {
-    const int c = g * w + i;
-    const double a = gamma ? gamma[c] * r : r;
-    scale[(long long)n * C + c] = (float)a;
-    shift[(long long)n * C + c] = (float)((beta ? beta[c] : 0.0) - m * a);
-    if (qs) {
-      qs[(long long)n * C + c] = (float)r;
-      qt[(long long)n * C + c] = (float)(-m * r);
-    }
-  }
-}
-
+// ------------------------------------------------------------------------------------------------ sums over a block
 // Threads in segments of `lanes`, a power of two up to 64 or a multiple of 64: the sums over a segment, in its first thread.
 // Every thread of the block calls; `waves` holds one entry per wave.
 struct Segments {
@@ -172,39 +38,71 @@ struct Segments {
   }
 };
 
-// The groups of a thread's 8 channels, the first of them `first` (a multiple of 8 in the slab).
-struct GroupWalk {
-  int g, left, width;
-  __device__ __forceinline__ GroupWalk(int first, int w) : width(w) {
-    g = first / w;
-    left = w - (first - g * w);
+// f(j, table[group of channel first + j]) for the 8 channels of a thread, `first` a multiple of 8 counted from a group's start.
+template <typename V, typename F>
+__device__ __forceinline__ void each_group(const V* table, int first, int width, F f) {
+  int g = first / width;
+  if ((width & 7) == 0) {
+    const V v = table[g];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f(j, v);
+    return;
   }
-  __device__ __forceinline__ void next() {
+  int left = width - (first - g * width);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    f(j, table[g]);
     if (--left == 0) {
       left = width;
       ++g;
     }
   }
-};
+}
 
-// Second halves of a reduction inside the pass that needs its result, where an image has few partial sums: every block adds
-// them up for itself, which saves a launch (5 us).  All channels are in one slab (C <= 512).
-// Per channel the sums over `blocks` of f(partial, block) as chan[c]; 256 threads.
+// Coefficients of z = x a + b for channels c.. of groups whose (mean, rstd) are in `stat`, the first channel being `first` there.
+__device__ __forceinline__ void affine_coef(float (&a)[8], float (&b)[8], const double2* stat, int first, int width,
+                                            const float* gamma, const float* beta, int c) {
+  load_param(a, gamma, c, 1.f);
+  load_param(b, beta, c, 0.f);
+  each_group(stat, first, width, [&](int j, double2 q) {
+    const double sc = a[j] * q.y;
+    a[j] = (float)sc;
+    b[j] = (float)(b[j] - q.x * sc);
+  });
+}
+// Of xhat = x s + t.
+__device__ __forceinline__ void unit_coef(float (&s)[8], float (&t)[8], const double2* stat, int first, int width) {
+  each_group(stat, first, width, [&](int j, double2 q) {
+    s[j] = (float)q.y;
+    t[j] = (float)(-q.x * q.y);
+  });
+}
+
+// Per column the sums over `blocks` of f(block, partial) as out[c], C columns of partials in rows of `pitch`; 256 threads.
+// Loads are issued by fours: the partials were written by other chiplets, and a round trip takes about a microsecond.
 template <typename F>
-__device__ __forceinline__ void channel_sums(double2* chan, double2* tree, int blocks, int C, F f) {
+__device__ __forceinline__ void column_sums(double2* out, double2* tree, const float2* part, int blocks, int C, int pitch,
+                                            F f) {
+  constexpr int U = 4;
   const int wide = C < kNormThreads ? C : kNormThreads, parts = kNormThreads / wide;
   const int i = threadIdx.x % wide, share = threadIdx.x / wide;
   for (int c0 = 0; c0 < C; c0 += wide) {
     const int c = c0 + i;
     double2 sum = make_double2(0, 0);
-    if (share < parts && c < C) {
-#pragma unroll 4
-      for (int k = share; k < blocks; k += parts) {
-        const double2 v = f(k, c);
-        sum.x += v.x;
-        sum.y += v.y;
+    if (share < parts && c < C)
+      for (int k0 = share; k0 < blocks; k0 += U * parts) {
+        float2 v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          v[u] = k0 + u * parts < blocks ? part[(long long)(k0 + u * parts) * pitch + c] : make_float2(0.f, 0.f);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (k0 + u * parts < blocks) {
+            const double2 t = f(k0 + u * parts, v[u]);
+            sum.x += t.x;
+            sum.y += t.y;
+          }
       }
-    }
     tree[threadIdx.x] = sum;
     __syncthreads();
     for (int left = parts; left > 1;) {
@@ -216,7 +114,7 @@ __device__ __forceinline__ void channel_sums(double2* chan, double2* tree, int b
       __syncthreads();
       left = half;
     }
-    if (share == 0 && c < C) chan[c] = tree[threadIdx.x];
+    if (share == 0 && c < C) out[c] = tree[threadIdx.x];
     __syncthreads();
   }
 }
@@ -244,7 +142,166 @@ __device__ __forceinline__ void group_sums(double2* group, const double2* chan, 
   }
   __syncthreads();
 }
-constexpr int kFewChannels = 512;
+constexpr int kSlabChannels = 512;                 // of norm_grid's widest slab
+
+// ------------------------------------------------------------------------------------------------ forward statistics
+// Per block and channel: mean and sum of squared differences from it.  A thread sums (x - k) and (x - k)^2 with k its own
+// first value, so that an offset of the channel that is large against its spread does not cancel; threads and blocks are
+// joined by counts, means and sums of squares.  A partial holds `join` channels: a group where slabs hold whole groups, else 1.
+template <typename T>
+__global__ __launch_bounds__(kNormThreads) void gn_stats_kernel(const char* x, long long xps, long long ximg, int pixels,
+                                                                int C, int join, NormGrid g, float2* __restrict__ part) {
+  constexpr int ES = Elem<T>::bytes, U = 4;
+  __shared__ double2 chan[kSlabChannels], group[kSlabChannels], waves[kNormThreads / 64];
+  __shared__ float lmean[kNormThreads * 8], lm2[kNormThreads * 8];
+  __shared__ int lcount[kNormThreads];
+  __shared__ double2 lsum[kNormThreads];
+  NormWalk w(g, blockIdx.x, pixels, C);
+  float k[8], s1[8], s2[8];
+  int count = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) k[j] = s1[j] = s2[j] = 0.f;
+  const int px = w.p0 + w.r;
+  if (w.active && px < w.p1) {
+    const char* xp = x + (w.n * ximg + px * xps + w.c) * ES;
+    const long long step = g.rows * xps * ES;
+    unpack8(k, load8<T>(xp));
+    auto sweep = [&](auto whole, int left) {
+      Vec8<T> v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (whole || u * g.rows < left) v[u] = load8<T>(xp + u * step);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (!whole && u * g.rows >= left) break;
+        float f[8];
+        unpack8(f, v[u]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float d = f[j] - k[j];
+          s1[j] += d;
+          s2[j] = fmaf(d, d, s2[j]);
+        }
+      }
+    };
+    for (int at = w.p0; at < w.p1; at += U * g.rows, xp += U * step) {
+      if (at + U * g.rows <= w.p1) sweep(WholeTag{}, 0);
+      else sweep(PartTag{}, w.p1 - at - w.r);
+    }
+    count = (w.p1 - px + g.rows - 1) / g.rows;
+  }
+  const float rc = count ? 1.f / (float)count : 0.f;
+  if ((int)threadIdx.x == w.r * g.cw) lcount[w.r] = count;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    lmean[threadIdx.x * 8 + j] = k[j] + s1[j] * rc;
+    lm2[threadIdx.x * 8 + j] = s2[j] - s1[j] * s1[j] * rc;
+  }
+  __syncthreads();
+  // channel i of the slab from `parts` threads, then from one
+  const int wide = g.cw * 8, parts = wide < kNormThreads ? kNormThreads / wide : 1;
+  for (int i0 = 0; i0 < wide; i0 += kNormThreads) {
+    const int i = i0 + (int)threadIdx.x % wide, q = (int)threadIdx.x / wide;
+    double sum = 0, sq = 0;
+    if (q < parts && i < wide)
+      for (int r = q; r < g.rows; r += parts) {
+        const double m = lmean[r * wide + i], n = lcount[r];
+        sum += n * m;
+        sq += lm2[r * wide + i] + n * m * m;
+      }
+    if (parts > 1) {
+      lsum[threadIdx.x] = make_double2(sum, sq);
+      __syncthreads();
+      if (q == 0)
+        for (int t = 1; t < parts; ++t) {
+          sum += lsum[t * wide + i].x;
+          sq += lsum[t * wide + i].y;
+        }
+    }
+    if (q == 0 && i < wide) chan[i] = make_double2(sum, sq);
+  }
+  __syncthreads();
+  const int c0 = blockIdx.y * wide, entries = (C - c0 < wide ? C - c0 : wide) / join;
+  const double2* from = chan;
+  if (join > 1) {
+    group_sums(group, chan, waves, entries, join);
+    from = group;
+  }
+  const double values = (double)(w.p1 - w.p0) * join;
+  for (int e = threadIdx.x; e < entries; e += kNormThreads) {
+    const double mean = from[e].x / values;
+    part[((long long)w.n * gridDim.x + blockIdx.x) * (C / join) + c0 / join + e] =
+        make_float2((float)mean, (float)(from[e].y - from[e].x * mean));
+  }
+}
+
+// Sum over the threads of a block, in every thread.
+template <int TB> __device__ __forceinline__ double block_sum(double v, double* lds) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = lds[0];
+#pragma unroll
+  for (int i = 1; i < TB / 64; ++i) v += lds[i];
+  return v;
+}
+
+constexpr int kFinThreads = 1024;
+
+// One block per (group, image): the blocks' statistics of the group's channels in 64 bits, then the coefficients.
+__global__ __launch_bounds__(kFinThreads) void gn_finalize_kernel(const float2* __restrict__ part, int blocks, int chunk,
+                                                                   long long pixels, int C, int groups, int join,
+                                                                   const float* __restrict__ gamma,
+                                                                   const float* __restrict__ beta, float eps,
+                                                                   float* __restrict__ mean, float* __restrict__ rstd,
+                                                                   float* __restrict__ scale, float* __restrict__ shift,
+                                                                   float* __restrict__ qs, float* __restrict__ qt) {
+  __shared__ double lds[kFinThreads / 64];
+  const int w = C / groups, g = blockIdx.x, n = blockIdx.y;
+  double s = 0, q = 0;
+  const int each = w / join, pitch = C / join, entries = blocks * each;
+  const int last = (int)(pixels - (long long)(blocks - 1) * chunk);
+  const float2* pp = part + (long long)n * blocks * pitch + g * each;
+  constexpr int U = 4;                             // loads in flight: the kernel waits for nothing else
+  for (int e0 = threadIdx.x; e0 < entries; e0 += U * kFinThreads) {
+    float2 v[U];
+    int count[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int e = e0 + u * kFinThreads, b = e / each;
+      count[u] = e >= entries ? 0 : b == blocks - 1 ? last : chunk;
+      v[u] = e < entries ? pp[(long long)b * pitch + (e - b * each)] : make_float2(0.f, 0.f);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const double n = (double)count[u] * join, m = v[u].x;
+      s += n * m;
+      q += (double)v[u].y + n * m * m;
+    }
+  }
+  s = block_sum<kFinThreads>(s, lds);
+  q = block_sum<kFinThreads>(q, lds);
+  const double count = (double)pixels * w, m = s / count;
+  double var = q / count - m * m;
+  if (var < 0) var = 0;
+  const double r = 1.0 / sqrt(var + (double)eps);
+  if (threadIdx.x == 0) {
+    mean[n * groups + g] = (float)m;
+    rstd[n * groups + g] = (float)r;
+  }
+  for (int i = threadIdx.x; i < w; i += kFinThreads) {
+    const int c = g * w + i;
+    const double a = gamma ? gamma[c] * r : r;
+    scale[(long long)n * C + c] = (float)a;
+    shift[(long long)n * C + c] = (float)((beta ? beta[c] : 0.0) - m * a);
+    if (qs) {
+      qs[(long long)n * C + c] = (float)r;
+      qt[(long long)n * C + c] = (float)(-m * r);
+    }
+  }
+}
 
 // ---------------------------------------------------------------------------- one pass: activated result, checkpoint
 // y = act(x a + b) and the checkpoint of x s + t (of x without s), either or both.  Coefficients per channel, `cimg` from
@@ -269,17 +326,16 @@ struct PassArgs {
   float eps;
 };
 
-// The statistics of the groups of image n out of the blocks' as (mean, rstd) in group[], and those of block 0 to memory.
+// The statistics of the groups of image n out of the blocks' (a partial a group) as (mean, rstd), and those of block 0 to
+// memory.  Every block adds them up for itself, which saves a launch.
 __device__ __forceinline__ void pass_statistics(const PassArgs& p, int n, double2* group) {
-  __shared__ double2 chan[kFewChannels], tree[kNormThreads], waves[kNormThreads / 64];
-  const float2* part = p.part + (long long)n * p.part_blocks * p.C;
+  __shared__ double2 tree[kNormThreads];
   const int last = p.pixels - (p.part_blocks - 1) * p.part_chunk, width = p.C / p.groups;
-  channel_sums(chan, tree, p.part_blocks, p.C, [&](int k, int c) {
-    const float2 v = part[k * p.C + c];
-    const double count = k == p.part_blocks - 1 ? last : p.part_chunk, m = v.x;
-    return make_double2(count * m, (double)v.y + count * m * m);
-  });
-  group_sums(group, chan, waves, p.groups, width);
+  column_sums(group, tree, p.part + (long long)n * p.part_blocks * p.groups, p.part_blocks, p.groups, p.groups,
+              [&](int k, float2 v) {
+                const double count = (double)(k == p.part_blocks - 1 ? last : p.part_chunk) * width, m = v.x;
+                return make_double2(count * m, (double)v.y + count * m * m);
+              });
   const double rcount = 1.0 / ((double)p.pixels * width);
   for (int g = threadIdx.x; g < p.groups; g += kNormThreads) {
     const double m = group[g].x * rcount;
@@ -301,19 +357,11 @@ __global__ __launch_bounds__(kNormThreads) void norm_pass_kernel(PassArgs p) {
   NormWalk w(p.g, gridDim.x - 1 - blockIdx.x, p.pixels, p.C);
   float a[8], b[8], s[8], t[8];
   if constexpr (FIN) {
-    __shared__ double2 group[kFewChannels];
+    __shared__ double2 group[kSlabChannels];
     pass_statistics(p, w.n, group);
     if (w.active) {
-      GroupWalk gw(w.c, p.C / p.groups);
-#pragma unroll
-      for (int j = 0; j < 8; ++j, gw.next()) {
-        const double2 q = group[gw.g];
-        const double sc = p.gamma ? p.gamma[w.c + j] * q.y : q.y;
-        a[j] = (float)sc;
-        b[j] = (float)((p.beta ? p.beta[w.c + j] : 0.0) - q.x * sc);
-        s[j] = (float)q.y;
-        t[j] = (float)(-q.x * q.y);
-      }
+      affine_coef(a, b, group, w.c, p.C / p.groups, p.gamma, p.beta, w.c);
+      if (Q) unit_coef(s, t, group, w.c, p.C / p.groups);
       if (blockIdx.x == 0 && w.r == 0) {
         store_coef(p.scale + (long long)w.n * p.C + w.c, a);
         store_coef(p.shift + (long long)w.n * p.C + w.c, b);
@@ -325,39 +373,50 @@ __global__ __launch_bounds__(kNormThreads) void norm_pass_kernel(PassArgs p) {
     if (Y) { load_coef(a, p.a + w.n * p.cimg + w.c); load_coef(b, p.b + w.n * p.cimg + w.c); }
     if (Q && p.s) { load_coef(s, p.s + w.n * p.cimg + w.c); load_coef(t, p.t + w.n * p.cimg + w.c); }
   }
+  if (!Q && !w.active) return;
   const int blocks32 = (p.C + 31) >> 5, rows = p.g.rows;
-  int px = w.p0 + w.r;
+  const int px = w.p0 + w.r;
   const char* xp = p.x + (w.n * p.ximg + px * p.xps + w.c) * ES;
   char* yp = p.y + (w.n * p.yimg + px * p.yps + w.c) * ES;
   const long long row = (long long)w.n * p.pixels + px, xstep = rows * p.xps * ES, ystep = rows * p.yps * ES;
   signed char* cp = p.codes + row * p.C + w.c;
   bf16_t* sp = p.scales + row * blocks32 + (w.c >> 5);
   const int cstep = rows * p.C, sstep = rows * blocks32;
-  for (; px < w.p1; px += U * rows) {
+  const bool first = w.active && (w.c & 31) == 0;
+  // left: pixels of this thread's column that are left; whole: all of a sweep's are there
+  auto sweep = [&](auto whole, int left) {
     Vec8<T> v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (w.active && px + u * rows < w.p1) v[u] = load8<T, true>(xp + u * xstep);
+      if ((!Q || w.active) && (whole || u * rows < left)) v[u] = load8<T, true>(xp + u * xstep);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (px + u * rows >= w.p1) break;
+      if (!whole && u * rows >= left) break;
       float f[8], o[8];
-      if (w.active) unpack8(f, v[u]);
-      if (Y && w.active) {
+      unpack8(f, v[u]);
+      if constexpr (Y) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) o[j] = act_fwd<ACT>(fmaf(f[j], a[j], b[j]));
-        store8<T, true>(yp + u * ystep, pack8<T>(o));
+        if (!Q || w.active) store8<T, true>(yp + u * ystep, pack8<T>(o));
       }
       if constexpr (Q) {
+        if (FIN || p.s) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] = !w.active ? 0.f : FIN || p.s ? fmaf(f[j], s[j], t[j]) : f[j];
-        const Quant8 q = quantise8(o);
-        if (w.active) {
-          *reinterpret_cast<uint2*>(cp + u * cstep) = q.codes;
-          if ((w.c & 31) == 0) sp[u * sstep] = q.scale;
+          for (int j = 0; j < 8; ++j) f[j] = fmaf(f[j], s[j], t[j]);
         }
+        if (!w.active) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) f[j] = 0.f;
+        }
+        const Quant8 q = quantise8(f);
+        if (w.active) *reinterpret_cast<uint2*>(cp + u * cstep) = q.codes;
+        if (first) sp[u * sstep] = q.scale;
       }
     }
+  };
+  for (int at = w.p0; at < w.p1; at += U * rows) {
+    if (at + U * rows <= w.p1) sweep(WholeTag{}, 0);
+    else sweep(PartTag{}, w.p1 - at - w.r);
     xp += U * xstep;
     yp += U * ystep;
     cp += U * cstep;
@@ -385,30 +444,34 @@ __global__ __launch_bounds__(kNormThreads) void checkpoint_read_kernel(ReadArgs 
   float a[8], b[8];
   if (AFF) { load_coef(a, p.a + w.n * p.cimg + w.c); load_coef(b, p.b + w.n * p.cimg + w.c); }
   const int blocks32 = (p.C + 31) >> 5, rows = p.g.rows;
-  int px = w.p0 + w.r;
+  const int px = w.p0 + w.r;
   const long long row = (long long)w.n * p.pixels + px, ystep = rows * p.yps * ES;
   const signed char* cp = p.codes + row * p.C + w.c;
   const bf16_t* sp = p.scales + row * blocks32 + (w.c >> 5);
   char* yp = p.y + (w.n * p.yimg + px * p.yps + w.c) * ES;
   const int cstep = rows * p.C, sstep = rows * blocks32;
-  for (; px < w.p1; px += U * rows) {
+  auto sweep = [&](auto whole, int left) {
     uint2 q[U];
     bf16_t s[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (px + u * rows < w.p1) {
+      if (whole || u * rows < left) {
         q[u] = load_codes<true>(cp + u * cstep);
         s[u] = sp[u * sstep];
       }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (px + u * rows >= w.p1) break;
+      if (!whole && u * rows >= left) break;
       float f[8];
       dequantise8(f, q[u], bf16_to_f32(s[u]));
 #pragma unroll
       for (int j = 0; j < 8; ++j) f[j] = act_fwd<ACT>(AFF ? fmaf(f[j], a[j], b[j]) : f[j]);
       store8<T, true>(yp + u * ystep, pack8<T>(f));
     }
+  };
+  for (int at = w.p0; at < w.p1; at += U * rows) {
+    if (at + U * rows <= w.p1) sweep(WholeTag{}, 0);
+    else sweep(PartTag{}, w.p1 - at - w.r);
     cp += U * cstep;
     sp += U * sstep;
     yp += U * ystep;
@@ -431,7 +494,7 @@ struct BwdArgs {
   long long xps, ximg, dps, dimg, ops, oimg;
   int pixels, C, groups, images;
   NormGrid g;
-  const float2* part;                              // FIN: the blocks' sums, `part_blocks` an image
+  const float2 *part, *gpart;                      // FIN: the blocks' sums a channel and a group, `part_blocks` an image
   int part_blocks;
 };
 
@@ -492,22 +555,21 @@ template <typename T, bool CK> struct BwdFrom {
 template <bool CK>
 __device__ __forceinline__ void bwd_coef(float (&za)[8], float (&zb)[8], const BwdArgs& p, const NormWalk& w) {
   if constexpr (CK) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      za[j] = p.gamma ? p.gamma[w.c + j] : 1.f;
-      zb[j] = p.beta ? p.beta[w.c + j] : 0.f;
-    }
+    load_param(za, p.gamma, w.c, 1.f);
+    load_param(zb, p.beta, w.c, 0.f);
   } else {
     load_coef(za, p.a + (long long)w.n * p.C + w.c);
     load_coef(zb, p.b + (long long)w.n * p.C + w.c);
   }
 }
 
-// First pass: per block and channel sum g and sum g xhat.  XNT: x does not stay in the caches, as it and dy together are more
+// First pass: per block and channel sum g and sum g xhat; with `gpart` (one slab) also per group, times the channels' a.  XNT: x does not stay in the caches, as it and dy together are more
 // than they hold.
 template <typename T, int ACT, bool CK, bool XNT>
-__global__ __launch_bounds__(kNormThreads) void gn_bwd_reduce_kernel(BwdArgs p, float2* __restrict__ part) {
+__global__ __launch_bounds__(kNormThreads) void gn_bwd_reduce_kernel(BwdArgs p, float2* __restrict__ part,
+                                                                     float2* __restrict__ gpart) {
   constexpr int U = 4;
+  __shared__ double2 chan[kSlabChannels], group[kSlabChannels], waves[kNormThreads / 64];
   __shared__ float l1[kNormThreads * 8], l2[kNormThreads * 8];
   __shared__ double2 lsum[kNormThreads];
   NormWalk w(p.g, blockIdx.x, p.pixels, p.C);
@@ -519,34 +581,34 @@ __global__ __launch_bounds__(kNormThreads) void gn_bwd_reduce_kernel(BwdArgs p, 
     bwd_coef<CK>(za, zb, p, w);
     if constexpr (!CK) {
       const int width = p.C / p.groups;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int at = w.n * p.groups + (w.c + j) / width;
-        m[j] = p.mean[at];
-        rs[j] = p.rstd[at];
-      }
+      each_group(p.mean + (long long)w.n * p.groups, w.c, width, [&](int j, float v) { m[j] = v; });
+      each_group(p.rstd + (long long)w.n * p.groups, w.c, width, [&](int j, float v) { rs[j] = v; });
     }
     BwdFrom<T, CK> from(p, w);
     const int rows = p.g.rows;
-    for (int px = w.p0 + w.r; px < w.p1; px += U * rows, from.next(U)) {
+    auto sweep = [&](auto whole, int left) {
       BwdLoad<T, CK> l[U];
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (px + u * rows < w.p1) from.template load<XNT, false>(l[u], u);
+        if (whole || u * rows < left) from.template load<XNT, false>(l[u], u);
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (px + u * rows < w.p1) {
-          float f[8], d[8];
-          unpack8(d, l[u].dy);
-          if constexpr (CK) dequantise8(f, l[u].codes, bf16_to_f32(l[u].scale));
-          else unpack8(f, l[u].x);
+      for (int u = 0; u < U; ++u) {
+        if (!whole && u * rows >= left) break;
+        float f[8], d[8];
+        unpack8(d, l[u].dy);
+        if constexpr (CK) dequantise8(f, l[u].codes, bf16_to_f32(l[u].scale));
+        else unpack8(f, l[u].x);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float gj = act_bwd<ACT>(fmaf(f[j], za[j], zb[j]), d[j]);
-            s1[j] += gj;
-            s2[j] = fmaf(gj, CK ? f[j] : f[j] - m[j], s2[j]);
-          }
+        for (int j = 0; j < 8; ++j) {
+          const float gj = act_bwd<ACT>(fmaf(f[j], za[j], zb[j]), d[j]);
+          s1[j] += gj;
+          s2[j] = fmaf(gj, CK ? f[j] : f[j] - m[j], s2[j]);
         }
+      }
+    };
+    for (int at = w.p0; at < w.p1; at += U * rows, from.next(U)) {
+      if (at + U * rows <= w.p1) sweep(WholeTag{}, 0);
+      else sweep(PartTag{}, w.p1 - at - w.r);
     }
     if constexpr (!CK) {
 #pragma unroll
@@ -578,8 +640,19 @@ __global__ __launch_bounds__(kNormThreads) void gn_bwd_reduce_kernel(BwdArgs p, 
         }
     }
     const int c = blockIdx.y * wide + i;
-    if (q == 0 && i < wide && c < p.C)
+    if (q == 0 && i < wide && c < p.C) {
       part[((long long)w.n * gridDim.x + blockIdx.x) * p.C + c] = make_float2((float)a, (float)b);
+      if (gpart) {
+        const double sc = p.a[(long long)w.n * p.C + c];
+        chan[c] = make_double2(sc * a, sc * b);
+      }
+    }
+  }
+  if (gpart) {
+    __syncthreads();
+    group_sums(group, chan, waves, p.groups, p.C / p.groups);
+    for (int g = threadIdx.x; g < p.groups; g += kNormThreads)
+      gpart[((long long)w.n * gridDim.x + blockIdx.x) * p.groups + g] = make_float2((float)group[g].x, (float)group[g].y);
   }
 }
 
@@ -588,7 +661,7 @@ __global__ __launch_bounds__(kNormThreads) void gn_bwd_finalize_kernel(BwdArgs p
                                                                        int ckpt, double2* __restrict__ sums, float* __restrict__ cm,
                                                                        float* __restrict__ cz, float* __restrict__ cp,
                                                                        float* __restrict__ cq) {
-  __shared__ double r1[kNormThreads], r2[kNormThreads], lds[4];
+  __shared__ double r1[kNormThreads], r2[kNormThreads], lds[kNormThreads / 64];
   const int w = p.C / p.groups, g = blockIdx.x, n = blockIdx.y;
   const int wide = w < kNormThreads ? w : kNormThreads, lanes = kNormThreads / wide;
   const int ci = threadIdx.x % wide, li = threadIdx.x / wide;
@@ -624,8 +697,8 @@ __global__ __launch_bounds__(kNormThreads) void gn_bwd_finalize_kernel(BwdArgs p
     __syncthreads();
   }
   const double count = (double)p.pixels * w;
-  k1 = block_sum(k1, lds) / count;
-  k2 = block_sum(k2, lds) / count;
+  k1 = block_sum<kNormThreads>(k1, lds) / count;
+  k2 = block_sum<kNormThreads>(k2, lds) / count;
   const float m = p.mean[n * p.groups + g], rs = p.rstd[n * p.groups + g];
   for (int i = threadIdx.x; i < w; i += kNormThreads) {
     const int c = g * w + i;
@@ -653,26 +726,28 @@ __device__ __forceinline__ void gn_bwd_params(const double2* sums, int images, i
 template <bool CK>
 __device__ __forceinline__ void group_bwd_coef(float (&za)[8], float (&zb)[8], float (&m)[8], float (&rs)[8], const BwdArgs& p,
                                                int n, int c, int width) {
-  const long long at = (long long)n * p.C + c;
   if constexpr (CK) {
+    load_param(za, p.gamma, c, 1.f);
+    load_param(zb, p.beta, c, 0.f);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      za[j] = p.gamma ? p.gamma[c + j] : 1.f;
-      zb[j] = p.beta ? p.beta[c + j] : 0.f;
       m[j] = 0.f;
       rs[j] = 1.f;
     }
   } else {
-    load_coef(za, p.a + at);
-    load_coef(zb, p.b + at);
-    GroupWalk gw(c, width);
-    gw.g += n * p.groups;
-#pragma unroll
-    for (int j = 0; j < 8; ++j, gw.next()) {
-      m[j] = p.mean[gw.g];
-      rs[j] = p.rstd[gw.g];
-    }
+    load_coef(za, p.a + (long long)n * p.C + c);
+    load_coef(zb, p.b + (long long)n * p.C + c);
+    each_group(p.mean + (long long)n * p.groups, c, width, [&](int j, float v) { m[j] = v; });
+    each_group(p.rstd + (long long)n * p.groups, c, width, [&](int j, float v) { rs[j] = v; });
   }
+}
+// kp and kq of the second pass from the groups' sums; kp holds rstd (1 for a checkpoint).
+__device__ __forceinline__ void share_coef(float (&kp)[8], float (&kq)[8], const double2* group, int first, int width, int pixels) {
+  const double rcount = 1.0 / ((double)pixels * width);
+  each_group(group, first, width, [&](int j, double2 k) {
+    kp[j] = (float)(-k.y * rcount * kp[j]);
+    kq[j] = (float)(-k.x * rcount);
+  });
 }
 
 template <typename T, int ACT, bool CK>
@@ -682,17 +757,17 @@ __device__ __forceinline__ void bwd_apply(const BwdArgs& p, const NormWalk& w, c
   constexpr int ES = Elem<T>::bytes, U = 4;
   BwdFrom<T, CK> from(p, w);
   const int rows = p.g.rows;
-  int px = w.p0 + w.r;
+  const int px = w.p0 + w.r;
   char* op = p.dx + (w.n * p.oimg + px * p.ops + w.c) * ES;
   const long long ostep = rows * p.ops * ES;
-  for (; px < w.p1; px += U * rows, from.next(U), op += U * ostep) {
+  auto sweep = [&](auto whole, int left) {
     BwdLoad<T, CK> l[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (px + u * rows < w.p1) from.template load<true, true>(l[u], u);
+      if (whole || u * rows < left) from.template load<true, true>(l[u], u);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (px + u * rows >= w.p1) break;
+      if (!whole && u * rows >= left) break;
       float f[8], d[8];
       unpack8(d, l[u].dy);
       if constexpr (CK) dequantise8(f, l[u].codes, bf16_to_f32(l[u].scale));
@@ -704,33 +779,34 @@ __device__ __forceinline__ void bwd_apply(const BwdArgs& p, const NormWalk& w, c
       }
       store8<T, true>(op + u * ostep, pack8<T>(d));
     }
+  };
+  for (int at = w.p0; at < w.p1; at += U * rows, from.next(U), op += U * ostep) {
+    if (at + U * rows <= w.p1) sweep(WholeTag{}, 0);
+    else sweep(PartTag{}, w.p1 - at - w.r);
   }
 }
 
+constexpr int kParamChannels = 16;                 // of a block that adds up the parameters' gradients
 // Second pass: dx = a g + (x - cm) cp + cq.  With dgamma or dbeta due, the blocks past the last pixels add them up.
-// FIN: the groups' sums out of the blocks'.
+// FIN: every block adds up the groups' sums of its image for itself, which saves a launch.
 template <typename T, int ACT, bool CK, bool FIN>
 __global__ __launch_bounds__(kNormThreads) void gn_bwd_apply_kernel(BwdArgs p) {
   if constexpr (FIN) {
-    __shared__ double2 chan[kFewChannels], group[kFewChannels], tree[kNormThreads], waves[kNormThreads / 64];
-    const bool params = (int)blockIdx.x == p.g.blocks;
-    if (params && blockIdx.z != 0) return;
-    const int n = blockIdx.z;
-    const float2* part = p.part + (long long)n * p.part_blocks * p.C;
-    channel_sums(chan, tree, params ? p.images * p.part_blocks : p.part_blocks, p.C, [&](int k, int c) {
-      const float2 v = part[k * p.C + c];
-      const double sc = params ? 1.0 : (double)p.a[(long long)n * p.C + c];
-      return make_double2(sc * v.x, sc * v.y);
-    });
-    if (params) {
-      for (int c = threadIdx.x; c < p.C; c += kNormThreads) {
-        if (p.dbeta) p.dbeta[c] = (float)chan[c].x;
-        if (p.dgamma) p.dgamma[c] = (float)chan[c].y;
+    __shared__ double2 group[kSlabChannels], tree[kNormThreads];
+    const auto plain = [](int, float2 v) { return make_double2(v.x, v.y); };
+    if ((int)blockIdx.x >= p.g.blocks) {
+      if (blockIdx.z != 0) return;
+      const int c0 = ((int)blockIdx.x - p.g.blocks) * kParamChannels;
+      const int channels = p.C - c0 < kParamChannels ? p.C - c0 : kParamChannels;
+      column_sums(group, tree, p.part + c0, p.images * p.part_blocks, channels, p.C, plain);
+      if ((int)threadIdx.x < channels) {
+        if (p.dbeta) p.dbeta[c0 + threadIdx.x] = (float)group[threadIdx.x].x;
+        if (p.dgamma) p.dgamma[c0 + threadIdx.x] = (float)group[threadIdx.x].y;
       }
       return;
     }
-    const int width = p.C / p.groups;
-    group_sums(group, chan, waves, p.groups, width);
+    const int n = blockIdx.z, width = p.C / p.groups;
+    column_sums(group, tree, p.gpart + (long long)n * p.part_blocks * p.groups, p.part_blocks, p.groups, p.groups, plain);
     NormWalk w(p.g, p.g.blocks - 1 - blockIdx.x, p.pixels, p.C);
     if (!w.active) return;
     float za[8], zb[8], a[8], m[8], kp[8], kq[8];
@@ -739,14 +815,7 @@ __global__ __launch_bounds__(kNormThreads) void gn_bwd_apply_kernel(BwdArgs p) {
     else
 #pragma unroll
       for (int j = 0; j < 8; ++j) a[j] = za[j];
-    const double rcount = 1.0 / ((double)p.pixels * width);
-    GroupWalk gw(w.c, width);
-#pragma unroll
-    for (int j = 0; j < 8; ++j, gw.next()) {
-      const double2 k = group[gw.g];
-      kp[j] = (float)(-k.y * rcount * kp[j]);
-      kq[j] = (float)(-k.x * rcount);
-    }
+    share_coef(kp, kq, group, w.c, width, p.pixels);
     bwd_apply<T, ACT, CK>(p, w, a, za, zb, m, kp, kq);
   } else {
     if ((int)blockIdx.x == p.g.blocks) {
@@ -912,14 +981,7 @@ __global__ __launch_bounds__(TB) void gn_small_fwd_kernel(SmallFwdArgs p) {
   __syncthreads();
   if (active) {
     float a[8], b[8];
-    GroupWalk gw(l * 8, width);
-#pragma unroll
-    for (int j = 0; j < 8; ++j, gw.next()) {
-      const double2 q = stat[gw.g];
-      const double sc = p.gamma ? p.gamma[c + j] * q.y : q.y;
-      a[j] = (float)sc;
-      b[j] = (float)((p.beta ? p.beta[c + j] : 0.0) - q.x * sc);
-    }
+    affine_coef(a, b, stat, l * 8, width, p.gamma, p.beta, c);
     if (r == 0) {
       store_coef(p.a + (long long)n * p.C + c, a);
       store_coef(p.b + (long long)n * p.C + c, b);
@@ -932,13 +994,7 @@ __global__ __launch_bounds__(TB) void gn_small_fwd_kernel(SmallFwdArgs p) {
   if constexpr (Q) {
     if (r >= rows) return;                        // whole quads of lanes: the others stay for the exchange in quantise8
     float qs[8], qt[8];
-    GroupWalk gw(active ? l * 8 : 0, width);
-#pragma unroll
-    for (int j = 0; j < 8; ++j, gw.next()) {
-      const double2 q = stat[gw.g < ng ? gw.g : 0];
-      qs[j] = (float)q.y;
-      qt[j] = (float)(-q.x * q.y);
-    }
+    unit_coef(qs, qt, stat, active ? l * 8 : 0, width);
     const int blocks32 = (p.C + 31) >> 5;
 #pragma unroll
     for (int u = 0; u < V; ++u) {
@@ -1092,20 +1148,13 @@ __global__ __launch_bounds__(TB) void gn_small_bwd_kernel(SmallBwdArgs q) {
   if (sg.seg < ng && sg.t == 0) tree[sg.seg] = sum;
   __syncthreads();
   if (!active) return;
-  const double rcount = 1.0 / ((double)p.pixels * width);
   float za[8], zb[8], m[8], a[8], kp[8], kq[8];   // read again rather than held over the exchange: registers are short
   group_bwd_coef<CK>(za, zb, m, kp, p, n, c, width);
   if constexpr (CK) load_coef(a, p.a + (long long)n * p.C + c);
   else
 #pragma unroll
     for (int j = 0; j < 8; ++j) a[j] = za[j];
-  GroupWalk gw(l * 8, width);
-#pragma unroll
-  for (int j = 0; j < 8; ++j, gw.next()) {
-    const double2 k = tree[gw.g];
-    kp[j] = (float)(-k.y * rcount * kp[j]);
-    kq[j] = (float)(-k.x * rcount);
-  }
+  share_coef(kp, kq, tree, l * 8, width, p.pixels);
   char* op = p.dx + (n * p.oimg + c) * ES;
   if (q.act == NA_RELU) small_bwd_finish<T, NA_RELU, CK, V>(op, p.ops, v, a, za, zb, m, kp, kq, r, rows, p.pixels);
   else if (q.act == NA_SILU) small_bwd_finish<T, NA_SILU, CK, V>(op, p.ops, v, a, za, zb, m, kp, kq, r, rows, p.pixels);
@@ -1202,11 +1251,11 @@ static int images_per_step(long long N, long long image_bytes) {
 
 // Whether an image's partial sums are few enough for every block of the second pass to add them up itself: 4096 of them
 // (32 KB), from blocks that read at most 192 KB each.
-constexpr int kFewEntries = 4096, kFewBlocks = 256, kFewPass = 1024;
+constexpr int kFewEntries = 4096, kFewBlocks = 256, kFewPass = 512;
 constexpr long long kFewBytes = 192 << 10;
-static bool few_partials(long long N, long long pixels, int C, int bytes, NormGrid& g) {
-  if (C > kFewChannels) return false;
-  const long long most = kFewEntries / C, spread = (kFewBlocks + N - 1) / N;
+static bool few_partials(long long N, long long pixels, int C, int groups, int bytes, NormGrid& g) {
+  if (C > kSlabChannels) return false;
+  const long long most = kFewEntries / groups, spread = (kFewBlocks + N - 1) / N;
   g = norm_grid(1, pixels, C, 1, 1);
   const long long deep = (pixels + 4 * g.rows - 1) / (4 * g.rows);     // blocks of the four sweeps that are in flight together
   const long long some = spread < most ? spread : most;
@@ -1238,7 +1287,8 @@ static long long gn_workspace(long long N, long long pixels, int C, int groups, 
   const long long part = gn_partials(N, pixels, C), coef = round_up(4LL * N * C), sums = 2 * round_up(8LL * N * C);
   if (!backward) return small_fwd(N, pixels, C, groups, dtype, checkpoint).threads ? 0 : part + (checkpoint ? 2 * coef : 0);
   if (small_bwd(N, pixels, C, groups, dtype).threads) return N > 1 ? sums : 0;
-  return sums + part + 4 * coef;
+  // the coefficients, or, where the second pass works them out for itself, the groups' partial sums (at most the channels')
+  return sums + part + (part > 4 * coef ? part : 4 * coef);
 }
 
 static void launch_pass(const PassArgs& p, int N, int storage, int act, hipStream_t s) {
@@ -1302,10 +1352,10 @@ int launch_group_norm_fwd(const miseg_group_norm_desc* d, hipStream_t s) {
     qs = (float*)ws;
     qt = (float*)(ws + round_up(4LL * d->N * d->C));
   }
-  if (NormGrid g; few_partials(d->N, d->pixels, d->C, bytes, g)) {
+  if (NormGrid g; few_partials(d->N, d->pixels, d->C, d->groups, bytes, g)) {
     by_type_act(storage, NA_NONE, [&](auto t, auto) {
       hipLaunchKernelGGL((gn_stats_kernel<decltype(t)>), dim3(g.blocks, g.ny, d->N), dim3(kNormThreads), 0, s,
-                         (const char*)d->x, (long long)d->x_pix, d->x_img, (int)d->pixels, d->C, g, part);
+                         (const char*)d->x, (long long)d->x_pix, d->x_img, (int)d->pixels, d->C, d->C / d->groups, g, part);
     });
     PassArgs p{(const char*)d->x, (char*)d->y, (signed char*)d->codes, (bf16_t*)d->code_scales, nullptr, nullptr, nullptr,
                nullptr, d->x_pix, d->x_img, d->y_pix, d->y_img, d->C, (int)d->pixels, d->C,
@@ -1321,12 +1371,13 @@ int launch_group_norm_fwd(const miseg_group_norm_desc* d, hipStream_t s) {
     const char* x = (const char*)d->x + n0 * d->x_img * bytes;
     const long long cat = (long long)n0 * d->C, gat = (long long)n0 * d->groups;
     const NormGrid g = norm_grid(n, d->pixels, d->C, kStatBlocks, kStatLeast);
+    const int width = d->C / d->groups, join = g.ny == 1 || g.cw * 8 % width == 0 ? width : 1;
     by_type_act(storage, NA_NONE, [&](auto t, auto) {
       hipLaunchKernelGGL((gn_stats_kernel<decltype(t)>), dim3(g.blocks, g.ny, n), dim3(kNormThreads), 0, s, x,
-                         (long long)d->x_pix, d->x_img, (int)d->pixels, d->C, g, part);
+                         (long long)d->x_pix, d->x_img, (int)d->pixels, d->C, join, g, part);
     });
-    hipLaunchKernelGGL(gn_finalize_kernel, dim3(d->groups, n), dim3(kNormThreads), 0, s, part, g.blocks, g.chunk, d->pixels,
-                       d->C, d->groups, d->gamma, d->beta, d->eps, d->mean + gat, d->rstd + gat, d->scale + cat,
+    hipLaunchKernelGGL(gn_finalize_kernel, dim3(d->groups, n), dim3(kFinThreads), 0, s, part, g.blocks, g.chunk, d->pixels,
+                       d->C, d->groups, join, d->gamma, d->beta, d->eps, d->mean + gat, d->rstd + gat, d->scale + cat,
                        d->shift + cat, qs, qt);
     PassArgs p{x, (char*)d->y + n0 * d->y_img * bytes, (signed char*)d->codes, (bf16_t*)d->code_scales, d->scale + cat,
                d->shift + cat, qs, qt, d->x_pix, d->x_img, d->y_pix, d->y_img, d->C, (int)d->pixels, d->C,
@@ -1398,10 +1449,11 @@ int launch_group_norm_bwd(const miseg_group_norm_bwd_desc* d, hipStream_t s) {
   const long long coef = round_up(4LL * d->N * d->C);
   float *cm = (float*)ws, *cz = (float*)(ws + coef), *cp = (float*)(ws + 2 * coef), *cq = (float*)(ws + 3 * coef);
   NormGrid few;
-  const bool fin = few_partials(d->N, d->pixels, d->C, bytes, few);
+  const bool fin = few_partials(d->N, d->pixels, d->C, d->groups, bytes, few);
   const long long dbytes = d->pixels * d->C * bytes, xbytes = ck ? d->pixels * (d->C + 2 * ((d->C + 31) / 32)) : dbytes;
   // both stay in the cache if they can; else dy alone; else the last pixels of both
   const bool alone = xbytes + dbytes > kCacheBytes && dbytes <= kCacheBytes;
+  float2* gpart = fin ? (float2*)cm : nullptr;     // the coefficients' place: there are none in memory then
   const int step = fin ? d->N : images_per_step(d->N, alone ? dbytes : xbytes + dbytes);
   for (int n0 = 0; n0 < d->N; n0 += step) {
     const int n = d->N - n0 < step ? d->N - n0 : step;
@@ -1410,7 +1462,7 @@ int launch_group_norm_bwd(const miseg_group_norm_bwd_desc* d, hipStream_t s) {
               (char*)d->dx + n0 * d->dx_img * bytes, (const signed char*)d->codes, (const bf16_t*)d->code_scales,
               d->mean + gat, d->rstd + gat, d->scale + cat, d->shift + cat, d->gamma, d->beta, cm, cz, cp, cq, nullptr,
               d->dgamma, d->dbeta, d->x_pix, d->x_img, d->dy_pix, d->dy_img, d->dx_pix, d->dx_img, (int)d->pixels, d->C,
-              d->groups, d->N, fin ? few : norm_grid(n, d->pixels, d->C, kStatBlocks, kStatLeast), part, few.blocks};
+              d->groups, d->N, fin ? few : norm_grid(n, d->pixels, d->C, kStatBlocks, kStatLeast), part, gpart, few.blocks};
     if (ck) {
       p.codes += n0 * d->pixels * d->C;
       p.scales += n0 * d->pixels * ((d->C + 31) / 32);
@@ -1420,10 +1472,10 @@ int launch_group_norm_bwd(const miseg_group_norm_bwd_desc* d, hipStream_t s) {
       typedef decltype(t) T;
       constexpr int A = decltype(a)::act;
       const dim3 grid(blocks, p.g.ny, n);
-      if (ck && alone) hipLaunchKernelGGL((gn_bwd_reduce_kernel<T, A, true, true>), grid, dim3(kNormThreads), 0, s, p, part);
-      else if (ck) hipLaunchKernelGGL((gn_bwd_reduce_kernel<T, A, true, false>), grid, dim3(kNormThreads), 0, s, p, part);
-      else if (alone) hipLaunchKernelGGL((gn_bwd_reduce_kernel<T, A, false, true>), grid, dim3(kNormThreads), 0, s, p, part);
-      else hipLaunchKernelGGL((gn_bwd_reduce_kernel<T, A, false, false>), grid, dim3(kNormThreads), 0, s, p, part);
+      if (ck && alone) hipLaunchKernelGGL((gn_bwd_reduce_kernel<T, A, true, true>), grid, dim3(kNormThreads), 0, s, p, part, gpart);
+      else if (ck) hipLaunchKernelGGL((gn_bwd_reduce_kernel<T, A, true, false>), grid, dim3(kNormThreads), 0, s, p, part, gpart);
+      else if (alone) hipLaunchKernelGGL((gn_bwd_reduce_kernel<T, A, false, true>), grid, dim3(kNormThreads), 0, s, p, part, gpart);
+      else hipLaunchKernelGGL((gn_bwd_reduce_kernel<T, A, false, false>), grid, dim3(kNormThreads), 0, s, p, part, gpart);
     });
     if (!fin)
       hipLaunchKernelGGL(gn_bwd_finalize_kernel, dim3(d->groups, n), dim3(kNormThreads), 0, s, p, part, blocks, ck ? 1 : 0,
@@ -1434,7 +1486,7 @@ int launch_group_norm_bwd(const miseg_group_norm_bwd_desc* d, hipStream_t s) {
     by_type_act(storage, act, [&](auto t, auto a) {
       typedef decltype(t) T;
       constexpr int A = decltype(a)::act;
-      const dim3 grid(p.g.blocks + (params ? 1 : 0), p.g.ny, n);
+      const dim3 grid(p.g.blocks + (!params ? 0 : fin ? (d->C + kParamChannels - 1) / kParamChannels : 1), p.g.ny, n);
       if (ck && fin) hipLaunchKernelGGL((gn_bwd_apply_kernel<T, A, true, true>), grid, dim3(kNormThreads), 0, s, p);
       else if (ck) hipLaunchKernelGGL((gn_bwd_apply_kernel<T, A, true, false>), grid, dim3(kNormThreads), 0, s, p);
       else if (fin) hipLaunchKernelGGL((gn_bwd_apply_kernel<T, A, false, true>), grid, dim3(kNormThreads), 0, s, p);

@@ -58,25 +58,46 @@ class Saved:
 
     def __init__(self, x, checkpoint, mean, rstd, scale, shift, gamma, beta, groups, act):
         self.x, self.checkpoint = x, checkpoint
-        self.stats, self.coefs = (mean, rstd), (scale, shift)
+        self._four, self._flat = (mean, rstd, scale, shift), None
         self.gamma, self.beta, self.groups, self.act = gamma, beta, groups, act
 
-    # `stats` and `coefs` are pairs, or tensors with one more dimension that are taken apart only where somebody asks
+    @classmethod
+    def _of(cls, x, checkpoint, flat, n, c, gamma, beta, groups, act):
+        """From the buffer of a forward call, scale, shift, mean, rstd one behind the other: taken apart where somebody asks."""
+        self = cls(x, checkpoint, None, None, None, None, gamma, beta, groups, act)
+        self._four, self._flat, self._n, self._c = None, flat, n, c
+        return self
+
+    def _part(self, which, columns, start):
+        return self._four[which] if self._four else self._flat.as_strided((self._n, columns), (columns, 1), start)
+
     @property
     def mean(self):
-        return self.stats[0]
+        return self._part(0, self.groups, 0 if self._four else 2 * self._n * self._c)
 
     @property
     def rstd(self):
-        return self.stats[1]
+        return self._part(1, self.groups, 0 if self._four else self._n * (2 * self._c + self.groups))
 
     @property
     def scale(self):
-        return self.coefs[0]
+        return self._part(2, 0 if self._four else self._c, 0)
 
     @property
     def shift(self):
-        return self.coefs[1]
+        return self._part(3, 0 if self._four else self._c, 0 if self._four else self._n * self._c)
+
+    def _addresses(self, n, c, device):
+        """Of mean, rstd, scale and shift, for an (n, ., ., c) tensor."""
+        g = self.groups
+        if self._flat is not None:
+            if (self._n, self._c) != (n, c) or self._flat.device != device:
+                raise L.MisegError("saved from %d images of %d channels on %s, not %d of %d on %s"
+                                   % (self._n, self._c, self._flat.device, n, c, device))
+            at = self._flat.data_ptr()
+            return at + 8 * n * c, at + 4 * n * (2 * c + g), at, at + 4 * n * c
+        return tuple(_coef(t, name, shape, device, False) for t, name, shape in
+                     zip(self._four, ("mean", "rstd", "scale", "shift"), ((n, g), (n, g), (n, c), (n, c))))
 
 
 def _view(t, name, like=None):
@@ -169,12 +190,10 @@ def group_norm_act(x, gamma, beta, groups, eps=1e-3, act="none", out=None, check
         if y.data_ptr() == d.x and not checkpoint:
             raise L.MisegError("out is x, which the backward pass needs: pass checkpoint=True or another tensor")
     d.y = y.data_ptr()
-    stats, coefs = x.new_empty((2, n, groups), dtype=torch.float32), x.new_empty((2, n, c), dtype=torch.float32)
+    flat = x.new_empty(2 * n * (c + groups), dtype=torch.float32)
     d.gamma, d.beta = _coef(gamma, "gamma", (c,), device), _coef(beta, "beta", (c,), device)
-    d.mean = at = stats.data_ptr()
-    d.rstd = at + 4 * n * groups
-    d.scale = at = coefs.data_ptr()
-    d.shift = at + 4 * n * c
+    d.scale = at = flat.data_ptr()
+    d.shift, d.mean, d.rstd = at + 4 * n * c, at + 8 * n * c, at + 4 * n * (2 * c + groups)
     ck = None
     if checkpoint:
         ck = Checkpoint8._like(x)
@@ -183,17 +202,7 @@ def group_norm_act(x, gamma, beta, groups, eps=1e-3, act="none", out=None, check
     d.dtype, d.fmt = _TYPES[dtype]
     ws = _workspace(lib, d, 1 if checkpoint else 0, 0, x)    # noqa: F841: lives until the launch is in its stream
     _launch(lib.miseg_group_norm_act_fwd, d, device)
-    saved = Saved(None if checkpoint else x, ck, None, None, None, None, gamma, beta, groups, act)
-    saved.stats, saved.coefs = stats, coefs
-    return y, saved
-
-
-def _pair_of(t, names, shape, device):
-    """Addresses of the two tensors of Saved.stats or Saved.coefs."""
-    if isinstance(t, torch.Tensor):
-        at = _coef(t, names[0], (2,) + shape, device, False)
-        return at, at + 4 * shape[0] * shape[1]
-    return _coef(t[0], names[0], shape, device, False), _coef(t[1], names[1], shape, device, False)
+    return y, Saved._of(None if checkpoint else x, ck, flat, n, c, gamma, beta, groups, act)
 
 
 def group_norm_act_backward(dy, saved, out=None):
@@ -226,8 +235,7 @@ def group_norm_act_backward(dy, saved, out=None):
         if dx.dtype != dtype:
             raise L.MisegError("out is %s, dy %s" % (dx.dtype, dtype))
     d.dx = dx.data_ptr()
-    d.mean, d.rstd = _pair_of(saved.stats, ("mean", "rstd"), (n, groups), device)
-    d.scale, d.shift = _pair_of(saved.coefs, ("scale", "shift"), (n, c), device)
+    d.mean, d.rstd, d.scale, d.shift = saved._addresses(n, c, device)
     d.gamma, d.beta = _coef(saved.gamma, "gamma", (c,), device), _coef(saved.beta, "beta", (c,), device)
     grads = dy.new_empty((2, c), dtype=torch.float32)
     d.dgamma = at = grads.data_ptr()
