@@ -101,6 +101,7 @@ class Model:
         self.loss = None
         self.metrics = []
         self.encoder_freeze = False
+        self.checkpoint_8bit = False       # set before the first fit(): activations kept in 8 bits (trainer.Trainer)
         self._engines = {}
         self._storage = "fp16"
 
@@ -296,7 +297,7 @@ class Model:
             t = trainer.Trainer(self.graph, self.weights, batch, device=self.device,
                                 learning_rate=opt.learning_rate, beta_1=opt.beta_1, beta_2=opt.beta_2,
                                 epsilon=opt.epsilon, loss=self._loss_name(), world_size=world,
-                                freeze_encoder=self.encoder_freeze)
+                                freeze_encoder=self.encoder_freeze, checkpoint_8bit=self.checkpoint_8bit)
             self._train_state = t
         elif t.n != batch:
             # parameters, optimiser state and BatchNorm scratch do not depend on the batch size and

@@ -24,6 +24,7 @@ import numpy as np
 import torch
 
 from . import lib as L
+from . import normops
 
 
 STAT_REPLICAS = 32
@@ -77,6 +78,14 @@ class Act:
         return v
 
 
+class Kept:
+    """An activation that the backward pass reads out of its 8-bit checkpoint: act(v * scale + shift) of its values v
+    (normops.checkpoint8_read), a tensor of c channels."""
+
+    def __init__(self, checkpoint, scale=None, shift=None, act="none"):
+        self.checkpoint, self.scale, self.shift, self.act = checkpoint, scale, shift, act
+
+
 class Seg:
     """One parameter tensor inside the flat buffers."""
 
@@ -87,7 +96,13 @@ class Seg:
 class Trainer:
     def __init__(self, graph, weights, batch, device="cuda:0", learning_rate=1e-3, beta_1=0.9, side_stream=True,
                  beta_2=0.999, epsilon=1e-7, loss="cce_dice", world_size=1, bucket_mb=25,
-                 freeze_encoder=False):
+                 freeze_encoder=False, checkpoint_8bit=False):
+        """checkpoint_8bit: what the backward pass needs of the forward pass is kept in 8.5 bits a value instead of 16
+        (normops.Checkpoint8), each 16-bit activation only until its last reader of the forward pass has run.  A
+        BatchNormalization + ReLU leaves the checkpoint of its normalised input, from which its own backward pass and the
+        operand of the next layer's weight gradient are worked out; other inputs of convolutions and poolings get a
+        checkpoint of their own.  The forward pass computes what it computes without; gradients see activations rounded to
+        1 / 254 of the largest of 32 neighbouring channels.  Not built for layers with a ReLU of their own (VGG)."""
         if not torch.cuda.is_available():
             raise L.MisegError("no GPU visible: the HIP training path has no CPU fallback")
         from .profile import TimedLib
@@ -112,6 +127,10 @@ class Trainer:
         self.focal = bool(self.loss_flags & L.LOSS_FOCAL)
         self.focal_alpha, self.focal_gamma = LS.FOCAL_ALPHA, LS.FOCAL_GAMMA
         self.world = world_size
+        self.checkpoint_8bit = bool(checkpoint_8bit)
+        if self.checkpoint_8bit and any(l.cls == "Conv2D" and l.config.get("activation") == "relu"
+                                        for l in graph.layers.values()):
+            raise NotImplementedError("8-bit checkpoints of a network whose convolutions have a ReLU of their own")
         # encoder_freeze (utils/model.py:179,191,203): the backbone's layers keep their weights and
         # their BatchNormalization layers run on the moving statistics
         self.frozen = set()
@@ -149,15 +168,31 @@ class Trainer:
                 if i not in self.place and g.layers[i].cls not in ("InputLayer", "ZeroPadding2D"):
                     self.place[i] = (l.name, c0)
                 c0 += c
-        self.head_up = self._fused_head_source()
-        self.fs = self._fused_final_stage()
-        self.p2 = self._folded_finest_level()
+        # with 8-bit checkpoints every layer runs as the graph states it: the folded forms keep tensors of their own
+        plain = self.checkpoint_8bit
+        self.head_up = None if plain else self._fused_head_source()
+        self.fs = None if plain else self._fused_final_stage()
+        self.p2 = None if plain else self._folded_finest_level()
+        self.drops = self._last_readers() if plain else {}
         self._ones = {}
         if self.fs is not None:
             # the aggregated buffer does not exist: its first input gets a tensor of its own
             for i in list(self.place):
                 if self.place[i][0] == self.fs["cat"]:
                     del self.place[i]
+
+    def _last_readers(self):
+        """Position in the graph's order -> the tensors whose last reader of the forward pass stands there."""
+        at = {n: i for i, n in enumerate(self.order)}
+        drops = {}
+
+        def last(name):
+            return max([max(at[c], last(c)) if self.g.layers[c].cls == "ZeroPadding2D" else at[c]
+                        for c in self.consumers[name]], default=-1)
+        for n in self.order:
+            if last(n) >= 0:
+                drops.setdefault(last(n), []).append(n)
+        return drops
 
     def _fused_head_source(self):
         """Name of the UpSampling2D(2, 'bilinear') whose only consumer is the 3x3 head convolution (the FPN
@@ -834,7 +869,7 @@ class Trainer:
         `relu_name` is read by exactly one layer and that layer runs on the persistent 32-channel kernel (a 3x3
         stride-1 convolution from 32 stored channels to at most 32, no fused addition): the two full-resolution
         layers at the end of the U-Net decoder, whose apply passes are the largest of the step."""
-        if os.environ.get("MISEG_NO_FWD_PROLOGUE") or xin.c != 32 or xin.c0 != 0 or xin.pix != 32:
+        if self.checkpoint_8bit or os.environ.get("MISEG_NO_FWD_PROLOGUE") or xin.c != 32 or xin.c0 != 0 or xin.pix != 32:
             return None
         cons = self.consumers.get(relu_name, [])
         if len(cons) != 1:
@@ -851,6 +886,62 @@ class Trainer:
         if self.fs is not None and r.name == self.fs["conv"] or self.p2 is not None and r.name == self.p2["conv"]:
             return None
         return r.name
+
+    def _keep(self, src, xin, reader):
+        """What layer `reader`'s backward pass will read of its input, tensor `src`: the tensor itself or its checkpoint."""
+        if not self.checkpoint_8bit:
+            return xin
+        if reader in self.frozen:
+            return None
+        kept = self.kept.get(src)
+        if kept is None:
+            kept = self.kept[src] = Kept(normops.checkpoint8_write(xin.t[..., xin.c0:xin.c0 + xin.c]))
+        return kept
+
+    def _operand(self, kept):
+        """The tensor behind what `_keep` returned."""
+        if not isinstance(kept, Kept):
+            return kept
+        n, h, w, c = kept.checkpoint.shape
+        out = self.new(h, w, c)
+        normops.checkpoint8_read(kept.checkpoint, kept.scale, kept.shift, act=kept.act, out=out.t[..., :c])
+        return out
+
+    def _bn_checkpoint_forward(self, l, relu, xin, s):
+        """BatchNormalization + ReLU in one pass that leaves the checkpoint of the normalised input: what the layer's own
+        backward pass reads (group normalisation of one image with a group a channel), and what the ReLU's readers take
+        their operands from."""
+        c, name = l.out.c, l.name
+        rstd = torch.rsqrt(s["var"][:c] + l.config["epsilon"])
+        gamma = self.view(name, "gamma") if l.config["scale"] else torch.ones_like(rstd)
+        beta = self.view(name, "beta")
+        out = self.new_out(relu, xin.h, xin.w, c)
+        ck, _ = normops.checkpoint8_write(xin.t[..., xin.c0:xin.c0 + c], rstd, -s["mean"][:c] * rstd, s["scale"][:c],
+                                          s["shift"][:c], act="relu", out=out.t[..., out.c0:out.c0 + c])
+        self.acts[relu] = out
+        self.kept[relu] = Kept(ck, gamma, beta, "relu")
+        rows = (1, xin.n * xin.h, xin.w)
+        flat = normops.Checkpoint8(ck.codes.view(*rows, c), ck.scales.view(*rows, ck.scales.shape[3]))
+        one = (1, c)
+        self.saved[name] = normops.Saved(None, flat, s["mean"][:c].view(one), rstd.view(one), s["scale"][:c].view(one),
+                                         s["shift"][:c].view(one), gamma, beta, c, "relu")
+
+    def _bn_checkpoint_backward(self, l, dy, grads):
+        c, name = l.out.c, l.name
+        rows = (1, dy.n * dy.h, dy.w)
+        out = self.new(dy.h, dy.w, c)
+        _, dgamma, dbeta = normops.group_norm_act_backward(dy.t.view(*rows, dy.pix)[..., dy.c0:dy.c0 + c],
+                                                           self.saved[name], out=out.t.view(*rows, out.pix)[..., :c])
+        self.gview(name, "beta").copy_(dbeta)
+        if l.config["scale"]:
+            self.gview(name, "gamma").copy_(dgamma)
+        self._accum(grads, l.inbound[0], out, name, dy)
+
+    def _drop_read(self, position):
+        """8-bit checkpoints: forgets the tensors whose last reader stands at `position`."""
+        for n in self.drops.get(position, ()):
+            self.acts.pop(n, None)
+            self.concat_bufs.pop(n, None)
 
     def _join_side(self):
         """The main stream waits for the weight gradients launched so far."""
@@ -931,6 +1022,7 @@ class Trainer:
         g, lib, st = self.g, self.lib, self.stream()
         self.acts = {}
         self.saved = {}
+        self.kept = {}                     # tensor -> its 8-bit checkpoint
         self.concat_bufs = {}
         self.fused_stats = set()
         self.fused_adds = set()
@@ -939,7 +1031,9 @@ class Trainer:
         self.fwd_prologues = set()      # BatchNormalizations whose apply pass the reading convolution does
         n = self.n
         self.x_in = x.contiguous()
-        for name in self.order:
+        for position, name in enumerate(self.order):
+            if position:
+                self._drop_read(position - 1)
             l = g.layers[name]
             cls = l.cls
             lib.tag = "fwd " + name
@@ -1010,7 +1104,7 @@ class Trainer:
                               l.out.w, bias=bias, act=act, probs=probs,
                               temperature=g.temperature if g.temperature else 1.0)
                     self.probs = probs
-                    self.saved[name] = (xin, pad)
+                    self.saved[name] = (self._keep(src, xin, name), pad)
                     continue
                 add = self._add_to_fuse(name) if not relu else None
                 if add is not None:
@@ -1023,7 +1117,7 @@ class Trainer:
                               bias=bias, residual=self.acts[other], stats=self._stats_for(add, co))
                     self.acts[add] = out
                     self.fused_adds.add(add)
-                    self.saved[name] = (xin, pad)
+                    self.saved[name] = (self._keep(src, xin, name), pad)
                     continue
                 out = self.new_out(name, l.out.h, l.out.w, co)
                 stats = None
@@ -1034,14 +1128,14 @@ class Trainer:
                 self.conv(xin, self.wptr(name), co, k, k, stride, stride, pad, pad, out, l.out.h, l.out.w,
                           bias=bias, stats=stats, act=L.ACT_RELU if relu else L.ACT_NONE)
                 self.acts[name] = out
-                self.saved[name] = (xin, pad)
+                self.saved[name] = (self._keep(src, xin, name), pad)
             elif cls == "Conv2DTranspose":
                 xin = self.acts[l.inbound[0]]
                 out = self.new_out(name, l.out.h, l.out.w, l.out.c)
                 self.conv(xin, self.wptr(name), l.out.c, 2, 2, 1, 1, 0, 0, out, xin.h, xin.w, transposed=True,
                           stats=self._stats_for(name, l.out.c))
                 self.acts[name] = out
-                self.saved[name] = (xin, 0)
+                self.saved[name] = (self._keep(l.inbound[0], xin, name), 0)
             elif cls == "BatchNormalization":
                 xin = self.acts[l.inbound[0]]
                 s = self.bn_state[name]
@@ -1092,6 +1186,9 @@ class Trainer:
                     g.layers[cons[0]].config["activation"] == "relu"
                 if not relu:
                     raise NotImplementedError("BatchNormalization without a following ReLU: %s" % name)
+                if self.checkpoint_8bit and name not in self.frozen:
+                    self._bn_checkpoint_forward(l, cons[0], xin, s)
+                    continue
                 if self._prologue_reader(cons[0], xin) is not None:
                     # the one reader applies scale/shift + ReLU to its operand tiles: no apply pass, no second tensor
                     self.acts[cons[0]] = Act(xin.t, c, xin.c0, pro=(s["scale"], s["shift"]))
@@ -1102,7 +1199,8 @@ class Trainer:
                                                            s["shift"].data_ptr(), xin.pixels, c, xin.pix,
                                                            out.pix, st))
                     self.acts[cons[0]] = out          # the ReLU's output
-                self.saved[name] = xin
+                if not self.checkpoint_8bit:
+                    self.saved[name] = xin
             elif cls == "Activation":
                 continue                           # relu: fused with its BatchNormalization; softmax: head
             elif cls == "TemperatureScaledSoftmax":
@@ -1118,7 +1216,7 @@ class Trainer:
                     L.check(lib.miseg_maxpool3x3s2_fwd(xin.ptr, out.ptr, None, None, n, xin.h, xin.w, xin.c,
                                                        xin.pix, out.pix, st))
                 self.acts[name] = out
-                self.saved[name] = xin
+                self.saved[name] = self._keep(src, xin, name)
             elif cls == "AveragePooling2D":
                 xin = self.acts[l.inbound[0]]
                 out = self.new_out(name, l.out.h, l.out.w, l.out.c)
@@ -1165,6 +1263,7 @@ class Trainer:
                 self.acts[name] = out
             else:
                 raise NotImplementedError("layer class %s" % cls)
+        self._drop_read(len(self.order) - 1)
         return self.probs
 
     def _frozen_bn(self, l, s):
@@ -1321,6 +1420,8 @@ class Trainer:
                 self._conv_backward(l, dy, grads)
             elif cls == "Conv2DTranspose":
                 self._convT_backward(l, dy, grads)
+            elif cls == "BatchNormalization" and self.checkpoint_8bit:
+                self._bn_checkpoint_backward(l, dy, grads)
             elif cls == "BatchNormalization":
                 xin = self.saved[name]
                 s = self.bn_state[name]
@@ -1350,7 +1451,7 @@ class Trainer:
                     self.gview(name, "gamma").copy_(sums[cc:])
                 self._fused_dgrad(grads, l.inbound[0], name, dy, run)
             elif cls == "MaxPooling2D":
-                xin = self.saved[name]
+                xin = self._operand(self.saved[name])
                 if l.config["pool_size"] == 2:
                     dx = self.new(xin.h, xin.w, xin.c)
                     L.check(lib.miseg_maxpool2x2_bwd(xin.ptr, dy.ptr, dx.ptr, n, xin.h, xin.w, xin.c, xin.pix,
@@ -1414,7 +1515,7 @@ class Trainer:
         only layer that reads it, the reader's data gradient can apply the ReLU's mask and gather the
         BatchNormalization's two backward reductions while it stores (one pass over x and the gradient less
         per BatchNormalization).  Returns the `bn_mask` argument of conv(), or None."""
-        if os.environ.get("MISEG_NO_FUSED_BN_BWD") or src_name in grads:
+        if self.checkpoint_8bit or os.environ.get("MISEG_NO_FUSED_BN_BWD") or src_name in grads:
             return None
         g = self.g
         relu = src_name
@@ -1524,6 +1625,7 @@ class Trainer:
                 self.grad_log[name] = (dy, None)
             return
         xin, pad = self.saved[name]
+        xin = self._operand(xin)
         cin = _c32(xin.c)
         self.wgrad(xin, dy.ptr, dy_str, dw_ptr, cin, (co + 7) // 8 * 8, k, k, stride, stride, pad, pad,
                    l.out.h, l.out.w, dy_t=dy.t)
@@ -1562,7 +1664,7 @@ class Trainer:
 
     def _convT_backward(self, l, dy, grads):
         name = l.name
-        xin, _ = self.saved[name]
+        xin = self._operand(self.saved[name][0])
         co = l.out.c
         cin = _c32(xin.c)
         seg = self.segs[(name, "kernel")]
