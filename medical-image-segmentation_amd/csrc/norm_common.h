@@ -106,8 +106,8 @@ template <int ACT> __device__ __forceinline__ float act_bwd(float z, float dy) {
 }
 
 // ---- pixels x channels over a grid: blockIdx = (pixel chunk, channel slab, image).  A slab is `cw` groups of 8
-// channels, a multiple of 4 so that the four lanes of a 32-channel block are neighbours; a block's 256 threads are
-// `rows` pixels x cw groups, and a thread keeps its 8 channels for its whole walk.
+// channels, at most 64 (a multiple of 4 where 32-channel blocks are written, so that their four lanes are neighbours); a
+// block's 256 threads are `rows` pixels x cw groups, and a thread keeps its 8 channels for its whole walk.
 constexpr int kNormThreads = 256;
 struct NormGrid {
   int cw, ny, rows;                                // groups of 8 channels per slab, slabs, pixels per sweep
@@ -115,11 +115,11 @@ struct NormGrid {
 };
 
 // Blocks enough to fill the chip (`want` in all), none with less than `least` sweeps unless there are few of them anyway.
-static inline NormGrid norm_grid(long long N, long long pixels, int C, int want, int least) {
+static inline NormGrid norm_grid(long long N, long long pixels, int C, int want, int least, bool whole32 = false) {
   NormGrid g;
-  const int c8 = ((C + 31) / 32) * 4;
+  const int unit = whole32 ? 4 : 1, c8 = (C / 8 + unit - 1) / unit * unit;
   g.ny = (c8 + 63) / 64;
-  g.cw = ((c8 + g.ny - 1) / g.ny + 3) / 4 * 4;
+  g.cw = ((c8 + g.ny - 1) / g.ny + unit - 1) / unit * unit;
   g.rows = kNormThreads / g.cw;
   const long long sweeps = (pixels + g.rows - 1) / g.rows, all = sweeps * N * g.ny;
   if (all < (long long)least * 1024) least = (int)(all / 1024) + 1;

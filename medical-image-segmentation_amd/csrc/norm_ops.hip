@@ -657,13 +657,14 @@ __global__ __launch_bounds__(kNormThreads) void gn_bwd_reduce_kernel(BwdArgs p, 
 }
 
 // One block per (group, image): the channels' sums over the blocks, then over the group, in 64 bits.
-__global__ __launch_bounds__(kNormThreads) void gn_bwd_finalize_kernel(BwdArgs p, const float2* __restrict__ part, int blocks,
+template <int TB>
+__global__ __launch_bounds__(TB) void gn_bwd_finalize_kernel(BwdArgs p, const float2* __restrict__ part, int blocks,
                                                                        int ckpt, double2* __restrict__ sums, float* __restrict__ cm,
                                                                        float* __restrict__ cz, float* __restrict__ cp,
                                                                        float* __restrict__ cq) {
-  __shared__ double r1[kNormThreads], r2[kNormThreads], lds[kNormThreads / 64];
+  __shared__ double r1[TB], r2[TB], lds[TB / 64];
   const int w = p.C / p.groups, g = blockIdx.x, n = blockIdx.y;
-  const int wide = w < kNormThreads ? w : kNormThreads, lanes = kNormThreads / wide;
+  const int wide = w < TB ? w : TB, lanes = TB / wide;
   const int ci = threadIdx.x % wide, li = threadIdx.x / wide;
   double k1 = 0, k2 = 0;
   for (int c0 = 0; c0 < w; c0 += wide) {
@@ -697,10 +698,10 @@ __global__ __launch_bounds__(kNormThreads) void gn_bwd_finalize_kernel(BwdArgs p
     __syncthreads();
   }
   const double count = (double)p.pixels * w;
-  k1 = block_sum<kNormThreads>(k1, lds) / count;
-  k2 = block_sum<kNormThreads>(k2, lds) / count;
+  k1 = block_sum<TB>(k1, lds) / count;
+  k2 = block_sum<TB>(k2, lds) / count;
   const float m = p.mean[n * p.groups + g], rs = p.rstd[n * p.groups + g];
-  for (int i = threadIdx.x; i < w; i += kNormThreads) {
+  for (int i = threadIdx.x; i < w; i += TB) {
     const int c = g * w + i;
     const long long at = (long long)n * p.C + c;
     cm[at] = !ckpt ? m : p.gamma ? p.gamma[c] : 1.f;
@@ -1250,9 +1251,9 @@ static int images_per_step(long long N, long long image_bytes) {
 }
 
 // Whether an image's partial sums are few enough for every block of the second pass to add them up itself: 4096 of them
-// (32 KB), from blocks that read at most 192 KB each.
-constexpr int kFewEntries = 4096, kFewBlocks = 256, kFewPass = 512;
-constexpr long long kFewBytes = 192 << 10;
+// (32 KB), from blocks that read at most 128 KB of x each.
+constexpr int kFewEntries = 4096, kFewBlocks = 512, kFewPass = 512;
+constexpr long long kFewBytes = 128 << 10;
 static bool few_partials(long long N, long long pixels, int C, int groups, int bytes, NormGrid& g) {
   if (C > kSlabChannels) return false;
   const long long most = kFewEntries / groups, spread = (kFewBlocks + N - 1) / N;
@@ -1359,7 +1360,7 @@ int launch_group_norm_fwd(const miseg_group_norm_desc* d, hipStream_t s) {
     });
     PassArgs p{(const char*)d->x, (char*)d->y, (signed char*)d->codes, (bf16_t*)d->code_scales, nullptr, nullptr, nullptr,
                nullptr, d->x_pix, d->x_img, d->y_pix, d->y_img, d->C, (int)d->pixels, d->C,
-               norm_grid(d->N, d->pixels, d->C, kFewPass, kPassLeast), part, g.blocks, g.chunk, d->groups, d->gamma, d->beta,
+               norm_grid(d->N, d->pixels, d->C, kFewPass, kPassLeast, d->codes != nullptr), part, g.blocks, g.chunk, d->groups, d->gamma, d->beta,
                d->mean, d->rstd, d->scale, d->shift, d->eps};
     launch_pass(p, d->N, storage, act_of(d->act), s);
     MISEG_CHECK_HIP(hipGetLastError());
@@ -1381,7 +1382,7 @@ int launch_group_norm_fwd(const miseg_group_norm_desc* d, hipStream_t s) {
                        d->shift + cat, qs, qt);
     PassArgs p{x, (char*)d->y + n0 * d->y_img * bytes, (signed char*)d->codes, (bf16_t*)d->code_scales, d->scale + cat,
                d->shift + cat, qs, qt, d->x_pix, d->x_img, d->y_pix, d->y_img, d->C, (int)d->pixels, d->C,
-               norm_grid(n, d->pixels, d->C, kPassBlocks, kPassLeast), nullptr, 0, 0, 0, nullptr, nullptr, nullptr, nullptr,
+               norm_grid(n, d->pixels, d->C, kPassBlocks, kPassLeast, d->codes != nullptr), nullptr, 0, 0, 0, nullptr, nullptr, nullptr, nullptr,
                nullptr, nullptr, 0.f};
     if (p.codes) {
       p.codes += n0 * d->pixels * d->C;
@@ -1477,8 +1478,12 @@ int launch_group_norm_bwd(const miseg_group_norm_bwd_desc* d, hipStream_t s) {
       else if (alone) hipLaunchKernelGGL((gn_bwd_reduce_kernel<T, A, false, true>), grid, dim3(kNormThreads), 0, s, p, part, gpart);
       else hipLaunchKernelGGL((gn_bwd_reduce_kernel<T, A, false, false>), grid, dim3(kNormThreads), 0, s, p, part, gpart);
     });
-    if (!fin)
-      hipLaunchKernelGGL(gn_bwd_finalize_kernel, dim3(d->groups, n), dim3(kNormThreads), 0, s, p, part, blocks, ck ? 1 : 0,
+    // 1024 threads where a group has many partials: 8 x 60 x 582 x 312 in 4 groups 10 us with 256
+    if (!fin && (long long)blocks * (d->C / d->groups) > 4096)
+      hipLaunchKernelGGL((gn_bwd_finalize_kernel<1024>), dim3(d->groups, n), dim3(1024), 0, s, p, part, blocks, ck ? 1 : 0,
+                         sums + cat, cm, cz, cp, cq);
+    else if (!fin)
+      hipLaunchKernelGGL((gn_bwd_finalize_kernel<256>), dim3(d->groups, n), dim3(256), 0, s, p, part, blocks, ck ? 1 : 0,
                          sums + cat, cm, cz, cp, cq);
     p.g = norm_grid(n, d->pixels, d->C, fin ? kFewPass : kPassBlocks, kPassLeast);
     const bool params = n0 + n == d->N && (d->dgamma || d->dbeta);
@@ -1514,7 +1519,7 @@ int launch_checkpoint8_write(const miseg_checkpoint8_desc* d, hipStream_t s) {
                   "checkpoint8_write: y must be a view like x, and be x, another channel range of its buffer or apart from it");
   PassArgs p{(const char*)d->x, (char*)d->y, (signed char*)d->codes, (bf16_t*)d->code_scales, d->y_a, d->y_b, d->code_a,
              d->code_b, d->x_pix, d->x_img, d->y_pix, d->y_img, d->coef_img, (int)d->pixels, d->C,
-             norm_grid(d->N, d->pixels, d->C, kPassBlocks, kPassLeast), nullptr, 0, 0, 0, nullptr, nullptr, nullptr, nullptr,
+             norm_grid(d->N, d->pixels, d->C, kPassBlocks, kPassLeast, true), nullptr, 0, 0, 0, nullptr, nullptr, nullptr, nullptr,
              nullptr, nullptr, 0.f};
   launch_pass(p, d->N, storage_of(d->dtype, d->fmt), act_of(d->act), s);
   MISEG_CHECK_HIP(hipGetLastError());
