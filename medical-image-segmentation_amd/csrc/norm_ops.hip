@@ -145,7 +145,8 @@ __device__ __forceinline__ void group_sums(double2* group, const double2* chan, 
 constexpr int kSlabChannels = 512;                 // of norm_grid's widest slab
 
 // ------------------------------------------------------------------------------------------------ forward statistics
-// Per block and channel: mean and sum of squared differences from it.  A thread sums (x - k) and (x - k)^2 with k its own
+// Bound by reading x: 157 MB in 29 us (5.4 TB/s).  512 blocks, two a CU, read as fast as 2048 and leave a quarter of the
+// partials (the finalisation of 960 x 1280 x 64 takes 5.6 us, 17 with 2048).  Per block and channel: mean and sum of squared differences from it.  A thread sums (x - k) and (x - k)^2 with k its own
 // first value, so that an offset of the channel that is large against its spread does not cancel; threads and blocks are
 // joined by counts, means and sums of squares.  A partial holds `join` channels: a group where slabs hold whole groups, else 1.
 template <typename T>
@@ -288,8 +289,8 @@ __global__ __launch_bounds__(kFinThreads) void gn_finalize_kernel(const float2* 
   if (var < 0) var = 0;
   const double r = 1.0 / sqrt(var + (double)eps);
   if (threadIdx.x == 0) {
-    mean[n * groups + g] = (float)m;
-    rstd[n * groups + g] = (float)r;
+    mean[(long long)n * groups + g] = (float)m;
+    rstd[(long long)n * groups + g] = (float)r;
   }
   for (int i = threadIdx.x; i < w; i += kFinThreads) {
     const int c = g * w + i;
@@ -307,7 +308,8 @@ __global__ __launch_bounds__(kFinThreads) void gn_finalize_kernel(const float2* 
 // y = act(x a + b) and the checkpoint of x s + t (of x without s), either or both.  Coefficients per channel, `cimg` from
 // one image's to the next's.  A block makes one sweep of U pixels per thread where there is work for 32768 blocks: short
 // blocks keep more loads and stores in flight than long walks (operand of 4 x 960 x 1280 x 64 out of 8 bits: 200 us with
-// 4096 blocks, 158 with 32768).  x is read for the last time here and y is read by another kernel: neither stays in the
+// 4096 blocks, 158 with 32768).  Bound by memory: 157 MB in, out of the memory-side cache, and 157 MB out in 46 us (6.8 TB/s);
+// with SiLU and the checkpoint (240 x 320 x 128, 4 images) 199 MB in 32 us, the vector units half busy.  x is read for the last time here and y is read by another kernel: neither stays in the
 // caches.  The last pixels come first, as they are the likeliest to be in the caches still.
 struct PassArgs {
   const char* x;
@@ -563,8 +565,9 @@ __device__ __forceinline__ void bwd_coef(float (&za)[8], float (&zb)[8], const B
   }
 }
 
-// First pass: per block and channel sum g and sum g xhat; with `gpart` (one slab) also per group, times the channels' a.  XNT: x does not stay in the caches, as it and dy together are more
-// than they hold.
+// First pass: per block and channel sum g and sum g xhat; with `gpart` (one slab) also per group, times the channels' a.
+// XNT: x does not stay in the caches, as it and dy together are more than they hold.  Bound by reading: 157 MB (two images of
+// 480 x 640 x 64, x and dy) in 30 us, 241 MB (codes and dy of 960 x 1280 x 64) in 41 us (5.9 TB/s).
 template <typename T, int ACT, bool CK, bool XNT>
 __global__ __launch_bounds__(kNormThreads) void gn_bwd_reduce_kernel(BwdArgs p, float2* __restrict__ part,
                                                                      float2* __restrict__ gpart) {
@@ -656,12 +659,12 @@ __global__ __launch_bounds__(kNormThreads) void gn_bwd_reduce_kernel(BwdArgs p, 
   }
 }
 
-// One block per (group, image): the channels' sums over the blocks, then over the group, in 64 bits.
+// One block per (group, image): the channels' sums over the blocks, then over the group, in 64 bits.  Latency: 5 us.
 template <int TB>
 __global__ __launch_bounds__(TB) void gn_bwd_finalize_kernel(BwdArgs p, const float2* __restrict__ part, int blocks,
-                                                                       int ckpt, double2* __restrict__ sums, float* __restrict__ cm,
-                                                                       float* __restrict__ cz, float* __restrict__ cp,
-                                                                       float* __restrict__ cq) {
+                                                              int ckpt, double2* __restrict__ sums,
+                                                              float* __restrict__ cm, float* __restrict__ cz,
+                                                              float* __restrict__ cp, float* __restrict__ cq) {
   __shared__ double r1[TB], r2[TB], lds[TB / 64];
   const int w = p.C / p.groups, g = blockIdx.x, n = blockIdx.y;
   const int wide = w < TB ? w : TB, lanes = TB / wide;
@@ -700,7 +703,7 @@ __global__ __launch_bounds__(TB) void gn_bwd_finalize_kernel(BwdArgs p, const fl
   const double count = (double)p.pixels * w;
   k1 = block_sum<TB>(k1, lds) / count;
   k2 = block_sum<TB>(k2, lds) / count;
-  const float m = p.mean[n * p.groups + g], rs = p.rstd[n * p.groups + g];
+  const float m = p.mean[(long long)n * p.groups + g], rs = p.rstd[(long long)n * p.groups + g];
   for (int i = threadIdx.x; i < w; i += TB) {
     const int c = g * w + i;
     const long long at = (long long)n * p.C + c;
@@ -790,6 +793,8 @@ __device__ __forceinline__ void bwd_apply(const BwdArgs& p, const NormWalk& w, c
 constexpr int kParamChannels = 16;                 // of a block that adds up the parameters' gradients
 // Second pass: dx = a g + (x - cm) cp + cq.  With dgamma or dbeta due, the blocks past the last pixels add them up.
 // FIN: every block adds up the groups' sums of its image for itself, which saves a launch.
+// Bound by memory: 157 MB out of the memory-side cache and 79 MB out in 34 us (6.9 TB/s); 84 MB of codes from HBM, 157 MB of
+// dy and 157 MB out in 59 us (6.8 TB/s; 75 with scalar loads of the parameters in every block).
 template <typename T, int ACT, bool CK, bool FIN>
 __global__ __launch_bounds__(kNormThreads) void gn_bwd_apply_kernel(BwdArgs p) {
   if constexpr (FIN) {
@@ -974,7 +979,7 @@ __global__ __launch_bounds__(TB) void gn_small_fwd_kernel(SmallFwdArgs p) {
     double var = sum.y * rcount - m * m;
     if (var < 0) var = 0;
     const double rs = 1.0 / sqrt(var + (double)p.eps);
-    const int at = n * p.groups + c0 / width + sg.seg;
+    const long long at = (long long)n * p.groups + c0 / width + sg.seg;
     p.mean[at] = (float)m;
     p.rstd[at] = (float)rs;
     stat[sg.seg] = make_double2(m, rs);
@@ -1209,15 +1214,16 @@ constexpr int kPassBlocks = 32768, kPassLeast = 4; // the same for a pass that o
 // pass to the second.
 constexpr long long kCacheBytes = 200000000;
 
-// Registers hold V vectors of 8 values a thread in blocks of 256 and 1024 threads.
+// Registers hold V vectors of 8 values a thread, in blocks of 256 threads or of 1024 (backward: 512, whose threads have twice
+// the registers: x, dy and the coefficients of 1024 spilled).
 template <typename T> struct SmallHold { static constexpr int fwd[2] = {8, 16}, bwd[2] = {4, 16}; };
 template <> struct SmallHold<f32s> { static constexpr int fwd[2] = {4, 8}, bwd[2] = {2, 8}; };
 
 static int gcd_int(int a, int b) { return b ? gcd_int(b, a % b) : a; }
 
 // One launch pays where few pixels meet few channels: a load of a slab narrower than a line keeps a lane for every line, so
-// a block's time grows with its pixels (fp32, 61 x 83 x 40 in slabs of 8: 17 us in one launch, 13 in three; bf16, 30 x 40 x
-// 512 backward: 11 us, 15 in three).  Slabs are the widest of whole groups and whole 8s (32s where 32-channel blocks are
+// a block's time grows with its pixels (fp32, 3 x 61 x 83 x 40 in slabs of 8: 17 us in one launch, 10 in two; bf16, 2 x 30 x
+// 40 x 512 backward: 11 us, 15 in three).  Slabs are the widest of whole groups and whole 8s (32s where 32-channel blocks are
 // written) that a block can hold, up to 64 channels, while 256 blocks are left.
 constexpr int kSmallPixels = 2048;
 static SmallGrid small_grid(long long N, long long pixels, int C, int groups, bool whole32, const int (&threads)[2],
@@ -1251,8 +1257,9 @@ static int images_per_step(long long N, long long image_bytes) {
 }
 
 // Whether an image's partial sums are few enough for every block of the second pass to add them up itself: 4096 of them
-// (32 KB), from blocks that read at most 128 KB of x each.
-constexpr int kFewEntries = 4096, kFewBlocks = 512, kFewPass = 512;
+// (32 KB), from blocks that read at most 128 KB of x each.  Two launches and no idle gap for three: 3 x 61 x 83 x 72 out of 8
+// bits 13 us on the GPU, 18 in three.
+constexpr int kFewEntries = 4096, kFewBlocks = 512, kFewPass = 1024;
 constexpr long long kFewBytes = 128 << 10;
 static bool few_partials(long long N, long long pixels, int C, int groups, int bytes, NormGrid& g) {
   if (C > kSlabChannels) return false;

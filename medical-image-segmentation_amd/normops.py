@@ -126,7 +126,7 @@ def _view(t, name, like=None):
 def _coef(t, name, shape, device, optional=True):
     if t is None and optional:
         return None
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or tuple(t.shape) != shape or \
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.shape != shape or \
             t.device != device or not t.is_contiguous():
         raise L.MisegError("%s has to be a dense float32 tensor %s on %s" % (name, shape, device))
     return t.data_ptr()

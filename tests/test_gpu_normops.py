@@ -585,3 +585,62 @@ def test_a_layer_chain_of_convolution_and_normalisation(ops):
     close(dx, wdx, tx)
     close(dgamma, wg, tg)
     close(dbeta, wb, tb)
+
+
+@pytest.mark.parametrize("shape", [(2, 9, 11, 72, 9), (2, 90, 80, 72, 9), (2, 500, 400, 72, 9), (1, 30, 31, 520, 5)], ids=str)
+def test_parameters_from_a_flat_buffer(ops, shape):
+    """Slices of one float32 buffer at odd offsets, as an optimiser's flat parameters are, give what aligned copies give."""
+    n, h, w, c, groups = shape
+    x, dy, gamma, beta = make(n, h, w, c, torch.bfloat16, seed=4)
+    flat = torch.cat([torch.zeros(1, device="cuda"), gamma, torch.zeros(2, device="cuda"), beta])
+    g, b = flat[1:1 + c], flat[3 + c:3 + 2 * c]
+    assert g.data_ptr() % 16 and b.data_ptr() % 16
+    for ck in (False, True):
+        y, s = ops.group_norm_act(x, g, b, groups, act="relu", checkpoint=ck)
+        yw, sw = ops.group_norm_act(x, gamma, beta, groups, act="relu", checkpoint=ck)
+        assert torch.equal(y, yw) and torch.equal(s.shift, sw.shift)
+        for got, want in zip(ops.group_norm_act_backward(dy, s), ops.group_norm_act_backward(dy, sw)):
+            assert torch.equal(got, want)
+
+
+def test_views_that_are_refused(ops):
+    """Slices that start or step off 16 bytes, strides of other layouts, broadcasts, overlaps, types and sizes that differ."""
+    from miseg_amd import lib as L
+    wide = torch.zeros((2, 6, 7, 160), dtype=torch.bfloat16, device="cuda")
+    x = wide[..., :64]
+    odd = torch.zeros((2, 6, 7, 68), dtype=torch.bfloat16, device="cuda")[..., :64]
+    bad = [wide[..., 4:68], odd, wide.permute(0, 3, 1, 2)[:, :6, :7, :7], wide[:, ::2, :, :64], wide[..., :60],
+           wide[:1, ..., :64].expand(2, 6, 7, 64), wide[..., :128:2], wide[:0, ..., :64], x.to(torch.float64)]
+    for t in bad:
+        with pytest.raises(L.MisegError):
+            ops.group_norm_act(t, None, None, 1)
+        with pytest.raises(L.MisegError):
+            ops.checkpoint8_write(t)
+    y, s = ops.group_norm_act(x, None, None, 8)
+    for t in bad[:6] + [x.float(), x[:1], wide[..., :56]]:
+        with pytest.raises(L.MisegError):
+            ops.group_norm_act_backward(t, s)
+        with pytest.raises(L.MisegError):
+            ops.group_norm_act(x, None, None, 8, out=t)
+    for out in (x, wide[..., 32:96], wide[:, :, :, 8:72]):
+        with pytest.raises(L.MisegError):
+            ops.group_norm_act(x, None, None, 8, out=out)
+    gamma = torch.zeros(64, device="cuda")
+    for g in (gamma[:32], gamma.double(), gamma.cpu(), torch.zeros(128, device="cuda")[::2]):
+        with pytest.raises(L.MisegError):
+            ops.group_norm_act(x, g, None, 8)
+    for groups in (0, 7, 128, 8.0, None):
+        with pytest.raises(L.MisegError):
+            ops.group_norm_act(x, None, None, groups)
+    with pytest.raises(L.MisegError):
+        ops.group_norm_act(x, None, None, 8, act="gelu")
+    with pytest.raises(L.MisegError):
+        ops.checkpoint8_write(x, gamma)
+    with pytest.raises(L.MisegError):
+        ops.checkpoint8_write(x, act="relu")
+    ck = ops.checkpoint8_write(x)
+    with pytest.raises(L.MisegError):
+        ops.checkpoint8_read(ck, out=wide[..., 4:68])
+    with pytest.raises(L.MisegError):
+        ops.checkpoint8_read(ck, dtype=torch.int8)
+    torch.cuda.synchronize()
