@@ -898,13 +898,15 @@ class Trainer:
             kept = self.kept[src] = Kept(normops.checkpoint8_write(xin.t[..., xin.c0:xin.c0 + xin.c]))
         return kept
 
-    def _operand(self, kept):
-        """The tensor behind what `_keep` returned."""
+    def _operand(self, kept, side=False):
+        """The tensor behind what `_keep` returned.  side: only weight gradients read it, so it is worked out on their stream
+        (which waits for the forward pass when the backward pass begins, and is waited for when it ends)."""
         if not isinstance(kept, Kept):
             return kept
         n, h, w, c = kept.checkpoint.shape
-        out = self.new(h, w, c)
-        normops.checkpoint8_read(kept.checkpoint, kept.scale, kept.shift, act=kept.act, out=out.t[..., :c])
+        with torch.cuda.stream(self.side if side else None):
+            out = self.new(h, w, c)
+            normops.checkpoint8_read(kept.checkpoint, kept.scale, kept.shift, act=kept.act, out=out.t[..., :c])
         return out
 
     def _bn_checkpoint_forward(self, l, relu, xin, s):
@@ -1625,7 +1627,7 @@ class Trainer:
                 self.grad_log[name] = (dy, None)
             return
         xin, pad = self.saved[name]
-        xin = self._operand(xin)
+        xin = self._operand(xin, side=True)
         cin = _c32(xin.c)
         self.wgrad(xin, dy.ptr, dy_str, dw_ptr, cin, (co + 7) // 8 * 8, k, k, stride, stride, pad, pad,
                    l.out.h, l.out.w, dy_t=dy.t)
@@ -1664,7 +1666,7 @@ class Trainer:
 
     def _convT_backward(self, l, dy, grads):
         name = l.name
-        xin = self._operand(self.saved[name][0])
+        xin = self._operand(self.saved[name][0], side=True)
         co = l.out.c
         cin = _c32(xin.c)
         seg = self.segs[(name, "kernel")]
