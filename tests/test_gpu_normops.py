@@ -644,3 +644,68 @@ def test_views_that_are_refused(ops):
     with pytest.raises(L.MisegError):
         ops.checkpoint8_read(ck, dtype=torch.int8)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("shape", [(2, 1, 3, 65536, 4096), (1, 3, 700, 65536, 1), (65535, 1, 1, 8, 2), (65535, 1, 2, 32, 32),
+                                   (1, 2100, 1, 520, 4), (1, 1, 2100, 1024, 8), (3, 47, 50, 8, 1)], ids=str)
+def test_extreme_extents(ops, shape):
+    n, h, w, c, groups = shape
+    dt, act = torch.bfloat16, "relu"
+    x, dy, gamma, beta = make(n, h, w, c, dt, seed=c)
+    for checkpoint in (False, True):
+        y, saved = ops.group_norm_act(x, gamma, beta, groups, act=act, checkpoint=checkpoint)
+        check_forward(x, y, saved, gamma, beta, groups, 1e-3, act)
+        dx, dgamma, dbeta = ops.group_norm_act_backward(dy, saved)
+        if checkpoint:
+            xhat = values(saved.checkpoint)
+            z = xhat * gamma.double() + beta.double()
+        else:
+            xhat = (x.double() - spread(saved.mean.double(), c)) * spread(saved.rstd.double(), c)
+            z = x.double() * saved.scale.double()[:, None, None] + saved.shift.double()[:, None, None]
+        wdx, wg, wb, tx, tg, tb = backward64(xhat, z, None, dy, saved.scale.double(), groups, act, dt)
+        close(dx, wdx, tx)
+        close(dgamma, wg, tg)
+        close(dbeta, wb, tb)
+
+
+def test_most_pixels(ops):
+    """23170 x 23170 pixels, just under the 2^29 that are allowed: statistics against sums in 64 bits, results against the
+    coefficients, a strip at a time."""
+    side, c = 23170, 8
+    x = torch.empty((1, side, side, c), dtype=torch.bfloat16, device="cuda")
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    strips = [slice(i, min(i + 2000, side)) for i in range(0, side, 2000)]
+    for s in strips:
+        x[:, s] = torch.randn((1, s.stop - s.start, side, c), generator=gen, device="cuda") + 0.5
+    gamma, beta = torch.randn(c, generator=gen, device="cuda"), torch.randn(c, generator=gen, device="cuda")
+    count = side * side * 4
+    mean = sum(x[:, s].double().reshape(-1, 2, 4).sum((0, 2)) for s in strips) / count
+    var = sum((x[:, s].double().reshape(-1, 2, 4) - mean[None, :, None]).square().sum((0, 2)) for s in strips) / count
+    y, saved = ops.group_norm_act(x, gamma, beta, 2, act="relu", checkpoint=True)
+    # 512 blocks of 256 rows of pixels: 4096 terms a thread instead of 64, their roundings of random sign: 64^0.5 = 8 times K
+    close(saved.mean[0], mean, 8 * K * U * torch.ones_like(mean))
+    close(saved.rstd[0], 1 / (var + 1e-3).sqrt(), 8 * K * U * torch.ones_like(mean))
+    a, b = saved.scale[0].double(), saved.shift[0].double()
+    for s in strips:
+        z = x[:, s].double() * a + b
+        close(y[:, s], z.clamp_min(0), half_step(y.dtype) * z.abs() + 4 * U * (z.abs() + b.abs()) + 1e-30)
+    dx, dgamma, dbeta = ops.group_norm_act_backward(torch.ones_like(y), saved)
+    s1 = torch.zeros(c, dtype=torch.float64, device="cuda")
+    s2 = torch.zeros(c, dtype=torch.float64, device="cuda")
+    for s in strips:
+        v = saved.checkpoint.codes[:, s].double() * saved.checkpoint.scales[:, s].double()
+        m = (v * gamma.double() + beta.double() > 0).double()
+        s1 += m.sum((0, 1, 2))
+        s2 += (m * v).sum((0, 1, 2))
+    # a thread's 4096 terms are counted exactly (dbeta), or at most 6 each in a running sum below 4096 * 6 (dgamma): each addition
+    # off by u times that; 131072 threads, random signs, 8 deviations
+    assert ((dbeta.double() - s1).abs() <= U * s1 + 1).all()
+    assert ((dgamma.double() - s2).abs() <= 8 * U * 4096 * 6 * (4096 * 131072.0) ** 0.5 + U * s2.abs()).all()
+    k1 = (a * s1).reshape(2, 4).sum(1).repeat_interleave(4) / count
+    k2 = (a * s2).reshape(2, 4).sum(1).repeat_interleave(4) / count
+    for s in strips[::4]:
+        v = saved.checkpoint.codes[:, s].double() * saved.checkpoint.scales[:, s].double()
+        m = (v * gamma.double() + beta.double() > 0).double()
+        want = a * m - k1 - v * k2
+        # k1 and k2 are known to the bound of the sums over the count
+        close(dx[:, s], want, half_step(dx.dtype) * want.abs() + 8 * U * a.abs().max() * (8 + v.abs()))
