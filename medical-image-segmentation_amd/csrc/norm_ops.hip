@@ -146,7 +146,7 @@ constexpr int kSlabChannels = 512;                 // of norm_grid's widest slab
 
 // ------------------------------------------------------------------------------------------------ forward statistics
 // Bound by reading x: 157 MB in 29 us (5.4 TB/s).  512 blocks, two a CU, read as fast as 2048 and leave a quarter of the
-// partials (the finalisation of 960 x 1280 x 64 takes 5.6 us, 17 with 2048).  Per block and channel: mean and sum of squared differences from it.  A thread sums (x - k) and (x - k)^2 with k its own
+// partials (the finalisation of 960 x 1280 x 64 takes 4.9 us, 17 with 2048).  Per block and channel: mean and sum of squared differences from it.  A thread sums (x - k) and (x - k)^2 with k its own
 // first value, so that an offset of the channel that is large against its spread does not cancel; threads and blocks are
 // joined by counts, means and sums of squares.  A partial holds `join` channels: a group where slabs hold whole groups, else 1.
 template <typename T>
@@ -249,29 +249,27 @@ template <int TB> __device__ __forceinline__ double block_sum(double v, double* 
   return v;
 }
 
-constexpr int kFinThreads = 1024;
-
 // One block per (group, image): the blocks' statistics of the group's channels in 64 bits, then the coefficients.
-__global__ __launch_bounds__(kFinThreads) void gn_finalize_kernel(const float2* __restrict__ part, int blocks, int chunk,
+__global__ __launch_bounds__(kNormThreads) void gn_finalize_kernel(const float2* __restrict__ part, int blocks, int chunk,
                                                                    long long pixels, int C, int groups, int join,
                                                                    const float* __restrict__ gamma,
                                                                    const float* __restrict__ beta, float eps,
                                                                    float* __restrict__ mean, float* __restrict__ rstd,
                                                                    float* __restrict__ scale, float* __restrict__ shift,
                                                                    float* __restrict__ qs, float* __restrict__ qt) {
-  __shared__ double lds[kFinThreads / 64];
+  __shared__ double lds[kNormThreads / 64];
   const int w = C / groups, g = blockIdx.x, n = blockIdx.y;
   double s = 0, q = 0;
   const int each = w / join, pitch = C / join, entries = blocks * each;
   const int last = (int)(pixels - (long long)(blocks - 1) * chunk);
   const float2* pp = part + (long long)n * blocks * pitch + g * each;
   constexpr int U = 4;                             // loads in flight: the kernel waits for nothing else
-  for (int e0 = threadIdx.x; e0 < entries; e0 += U * kFinThreads) {
+  for (int e0 = threadIdx.x; e0 < entries; e0 += U * kNormThreads) {
     float2 v[U];
     int count[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int e = e0 + u * kFinThreads, b = e / each;
+      const int e = e0 + u * kNormThreads, b = e / each;
       count[u] = e >= entries ? 0 : b == blocks - 1 ? last : chunk;
       v[u] = e < entries ? pp[(long long)b * pitch + (e - b * each)] : make_float2(0.f, 0.f);
     }
@@ -282,8 +280,8 @@ __global__ __launch_bounds__(kFinThreads) void gn_finalize_kernel(const float2* 
       q += (double)v[u].y + n * m * m;
     }
   }
-  s = block_sum<kFinThreads>(s, lds);
-  q = block_sum<kFinThreads>(q, lds);
+  s = block_sum<kNormThreads>(s, lds);
+  q = block_sum<kNormThreads>(q, lds);
   const double count = (double)pixels * w, m = s / count;
   double var = q / count - m * m;
   if (var < 0) var = 0;
@@ -292,7 +290,7 @@ __global__ __launch_bounds__(kFinThreads) void gn_finalize_kernel(const float2* 
     mean[(long long)n * groups + g] = (float)m;
     rstd[(long long)n * groups + g] = (float)r;
   }
-  for (int i = threadIdx.x; i < w; i += kFinThreads) {
+  for (int i = threadIdx.x; i < w; i += kNormThreads) {
     const int c = g * w + i;
     const double a = gamma ? gamma[c] * r : r;
     scale[(long long)n * C + c] = (float)a;
@@ -1384,7 +1382,7 @@ int launch_group_norm_fwd(const miseg_group_norm_desc* d, hipStream_t s) {
       hipLaunchKernelGGL((gn_stats_kernel<decltype(t)>), dim3(g.blocks, g.ny, n), dim3(kNormThreads), 0, s, x,
                          (long long)d->x_pix, d->x_img, (int)d->pixels, d->C, join, g, part);
     });
-    hipLaunchKernelGGL(gn_finalize_kernel, dim3(d->groups, n), dim3(kFinThreads), 0, s, part, g.blocks, g.chunk, d->pixels,
+    hipLaunchKernelGGL(gn_finalize_kernel, dim3(d->groups, n), dim3(kNormThreads), 0, s, part, g.blocks, g.chunk, d->pixels,
                        d->C, d->groups, join, d->gamma, d->beta, d->eps, d->mean + gat, d->rstd + gat, d->scale + cat,
                        d->shift + cat, qs, qt);
     PassArgs p{x, (char*)d->y + n0 * d->y_img * bytes, (signed char*)d->codes, (bf16_t*)d->code_scales, d->scale + cat,
