@@ -59,7 +59,7 @@ __device__ __forceinline__ void each_group(const V* table, int first, int width,
   }
 }
 
-// Coefficients of z = x a + b for channels c.. of groups whose (mean, rstd) are in `stat`, the first channel being `first` there.
+// Coefficients of z = x a + b for channels c.. of groups whose (mean, rstd) are in `stat`, where channel c is number `first`.
 __device__ __forceinline__ void affine_coef(float (&a)[8], float (&b)[8], const double2* stat, int first, int width,
                                             const float* gamma, const float* beta, int c) {
   load_param(a, gamma, c, 1.f);
@@ -145,10 +145,11 @@ __device__ __forceinline__ void group_sums(double2* group, const double2* chan, 
 constexpr int kSlabChannels = 512;                 // of norm_grid's widest slab
 
 // ------------------------------------------------------------------------------------------------ forward statistics
-// Bound by reading x: 157 MB in 29 us (5.4 TB/s).  512 blocks, two a CU, read as fast as 2048 and leave a quarter of the
-// partials (the finalisation of 960 x 1280 x 64 takes 4.9 us, 17 with 2048).  Per block and channel: mean and sum of squared differences from it.  A thread sums (x - k) and (x - k)^2 with k its own
+// Per block and channel: mean and sum of squared differences from it.  A thread sums (x - k) and (x - k)^2 with k its own
 // first value, so that an offset of the channel that is large against its spread does not cancel; threads and blocks are
 // joined by counts, means and sums of squares.  A partial holds `join` channels: a group where slabs hold whole groups, else 1.
+// Bound by reading x: 157 MB in 30 us (5.3 TB/s).  512 blocks, two a CU, read as fast as 2048 and leave a quarter of the
+// partials: the finalisation of 960 x 1280 x 64 takes 4.9 us, 17 with 2048.
 template <typename T>
 __global__ __launch_bounds__(kNormThreads) void gn_stats_kernel(const char* x, long long xps, long long ximg, int pixels,
                                                                 int C, int join, NormGrid g, float2* __restrict__ part) {
@@ -306,9 +307,10 @@ __global__ __launch_bounds__(kNormThreads) void gn_finalize_kernel(const float2*
 // y = act(x a + b) and the checkpoint of x s + t (of x without s), either or both.  Coefficients per channel, `cimg` from
 // one image's to the next's.  A block makes one sweep of U pixels per thread where there is work for 32768 blocks: short
 // blocks keep more loads and stores in flight than long walks (operand of 4 x 960 x 1280 x 64 out of 8 bits: 200 us with
-// 4096 blocks, 158 with 32768).  Bound by memory: 157 MB in, out of the memory-side cache, and 157 MB out in 46 us (6.8 TB/s);
-// with SiLU and the checkpoint (240 x 320 x 128, 4 images) 199 MB in 32 us, the vector units half busy.  x is read for the last time here and y is read by another kernel: neither stays in the
+// 4096 blocks, 158 with 32768).  x is read for the last time here and y is read by another kernel: neither stays in the
 // caches.  The last pixels come first, as they are the likeliest to be in the caches still.
+// Bound by memory: 157 MB in, out of the memory-side cache, and 157 MB out in 46 us (6.8 TB/s); with the checkpoint (4 x 240
+// x 320 x 128) 199 MB in 31 us (6.4 TB/s), with SiLU as without.
 struct PassArgs {
   const char* x;
   char* y;
@@ -319,11 +321,11 @@ struct PassArgs {
   int pixels, C;
   NormGrid g;
   // FIN: group normalisation out of the partial statistics
-  const float2* part;
-  int part_blocks, part_chunk, groups;
-  const float *gamma, *beta;
-  float *mean, *rstd, *scale, *shift;
-  float eps;
+  const float2* part = nullptr;
+  int part_blocks = 0, part_chunk = 0, groups = 0;
+  const float *gamma = nullptr, *beta = nullptr;
+  float *mean = nullptr, *rstd = nullptr, *scale = nullptr, *shift = nullptr;
+  float eps = 0.f;
 };
 
 // The statistics of the groups of image n out of the blocks' (a partial a group) as (mean, rstd), and those of block 0 to
@@ -1365,8 +1367,8 @@ int launch_group_norm_fwd(const miseg_group_norm_desc* d, hipStream_t s) {
     });
     PassArgs p{(const char*)d->x, (char*)d->y, (signed char*)d->codes, (bf16_t*)d->code_scales, nullptr, nullptr, nullptr,
                nullptr, d->x_pix, d->x_img, d->y_pix, d->y_img, d->C, (int)d->pixels, d->C,
-               norm_grid(d->N, d->pixels, d->C, kFewPass, kPassLeast, d->codes != nullptr), part, g.blocks, g.chunk, d->groups, d->gamma, d->beta,
-               d->mean, d->rstd, d->scale, d->shift, d->eps};
+               norm_grid(d->N, d->pixels, d->C, kFewPass, kPassLeast, d->codes != nullptr), part, g.blocks, g.chunk,
+               d->groups, d->gamma, d->beta, d->mean, d->rstd, d->scale, d->shift, d->eps};
     launch_pass(p, d->N, storage, act_of(d->act), s);
     MISEG_CHECK_HIP(hipGetLastError());
     return MISEG_OK;
@@ -1387,8 +1389,7 @@ int launch_group_norm_fwd(const miseg_group_norm_desc* d, hipStream_t s) {
                        d->shift + cat, qs, qt);
     PassArgs p{x, (char*)d->y + n0 * d->y_img * bytes, (signed char*)d->codes, (bf16_t*)d->code_scales, d->scale + cat,
                d->shift + cat, qs, qt, d->x_pix, d->x_img, d->y_pix, d->y_img, d->C, (int)d->pixels, d->C,
-               norm_grid(n, d->pixels, d->C, kPassBlocks, kPassLeast, d->codes != nullptr), nullptr, 0, 0, 0, nullptr, nullptr, nullptr, nullptr,
-               nullptr, nullptr, 0.f};
+               norm_grid(n, d->pixels, d->C, kPassBlocks, kPassLeast, d->codes != nullptr)};
     if (p.codes) {
       p.codes += n0 * d->pixels * d->C;
       p.scales += n0 * d->pixels * ((d->C + 31) / 32);
@@ -1429,7 +1430,7 @@ int launch_group_norm_bwd(const miseg_group_norm_bwd_desc* d, hipStream_t s) {
     SmallBwdArgs q{{(const char*)d->x, (const char*)d->dy, (char*)d->dx, (const signed char*)d->codes,
                     (const bf16_t*)d->code_scales, d->mean, d->rstd, d->scale, d->shift, d->gamma, d->beta, nullptr, nullptr,
                     nullptr, nullptr, nullptr, d->dgamma, d->dbeta, d->x_pix, d->x_img, d->dy_pix, d->dy_img, d->dx_pix,
-                    d->dx_img, (int)d->pixels, d->C, d->groups, d->N, NormGrid{}},
+                    d->dx_img, (int)d->pixels, d->C, d->groups, d->N, NormGrid{}, nullptr, nullptr, 0},
                    sums, act, d->N * sg.slabs, sg};
     const dim3 grid(q.blocks), block(sg.threads);
     by_type_act(storage, NA_NONE, [&](auto t, auto) {
@@ -1454,7 +1455,7 @@ int launch_group_norm_bwd(const miseg_group_norm_bwd_desc* d, hipStream_t s) {
   ws += gn_partials(d->N, d->pixels, d->C);
   const long long coef = round_up(4LL * d->N * d->C);
   float *cm = (float*)ws, *cz = (float*)(ws + coef), *cp = (float*)(ws + 2 * coef), *cq = (float*)(ws + 3 * coef);
-  NormGrid few;
+  NormGrid few{};
   const bool fin = few_partials(d->N, d->pixels, d->C, d->groups, bytes, few);
   const long long dbytes = d->pixels * d->C * bytes, xbytes = ck ? d->pixels * (d->C + 2 * ((d->C + 31) / 32)) : dbytes;
   // both stay in the cache if they can; else dy alone; else the last pixels of both
@@ -1477,11 +1478,11 @@ int launch_group_norm_bwd(const miseg_group_norm_bwd_desc* d, hipStream_t s) {
     by_type_act(storage, act, [&](auto t, auto a) {
       typedef decltype(t) T;
       constexpr int A = decltype(a)::act;
-      const dim3 grid(blocks, p.g.ny, n);
-      if (ck && alone) hipLaunchKernelGGL((gn_bwd_reduce_kernel<T, A, true, true>), grid, dim3(kNormThreads), 0, s, p, part, gpart);
-      else if (ck) hipLaunchKernelGGL((gn_bwd_reduce_kernel<T, A, true, false>), grid, dim3(kNormThreads), 0, s, p, part, gpart);
-      else if (alone) hipLaunchKernelGGL((gn_bwd_reduce_kernel<T, A, false, true>), grid, dim3(kNormThreads), 0, s, p, part, gpart);
-      else hipLaunchKernelGGL((gn_bwd_reduce_kernel<T, A, false, false>), grid, dim3(kNormThreads), 0, s, p, part, gpart);
+      const dim3 grid(blocks, p.g.ny, n), block(kNormThreads);
+      if (ck && alone) hipLaunchKernelGGL((gn_bwd_reduce_kernel<T, A, true, true>), grid, block, 0, s, p, part, gpart);
+      else if (ck) hipLaunchKernelGGL((gn_bwd_reduce_kernel<T, A, true, false>), grid, block, 0, s, p, part, gpart);
+      else if (alone) hipLaunchKernelGGL((gn_bwd_reduce_kernel<T, A, false, true>), grid, block, 0, s, p, part, gpart);
+      else hipLaunchKernelGGL((gn_bwd_reduce_kernel<T, A, false, false>), grid, block, 0, s, p, part, gpart);
     });
     // 1024 threads where a group has many partials: 8 x 60 x 582 x 312 in 4 groups 10 us with 256
     if (!fin && (long long)blocks * (d->C / d->groups) > 4096)
@@ -1524,8 +1525,7 @@ int launch_checkpoint8_write(const miseg_checkpoint8_desc* d, hipStream_t s) {
                   "checkpoint8_write: y must be a view like x, and be x, another channel range of its buffer or apart from it");
   PassArgs p{(const char*)d->x, (char*)d->y, (signed char*)d->codes, (bf16_t*)d->code_scales, d->y_a, d->y_b, d->code_a,
              d->code_b, d->x_pix, d->x_img, d->y_pix, d->y_img, d->coef_img, (int)d->pixels, d->C,
-             norm_grid(d->N, d->pixels, d->C, kPassBlocks, kPassLeast, true), nullptr, 0, 0, 0, nullptr, nullptr, nullptr, nullptr,
-             nullptr, nullptr, 0.f};
+             norm_grid(d->N, d->pixels, d->C, kPassBlocks, kPassLeast, true)};
   launch_pass(p, d->N, storage_of(d->dtype, d->fmt), act_of(d->act), s);
   MISEG_CHECK_HIP(hipGetLastError());
   return MISEG_OK;
