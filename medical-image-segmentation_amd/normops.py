@@ -5,7 +5,8 @@ batch statistics only): `group_norm_act` and `group_norm_act_backward` for batch
 `checkpoint8_write` / `checkpoint8_read`, which keep an activation for the backward pass in 8.5 bits a value.
 
 Tensors are (N, H, W, C) with C a multiple of 8, in bfloat16, float16 or float32, dense or a channel slice of a wider
-dense tensor that starts at a multiple of 16 bytes.  Every function launches on the current stream of its tensors' device.
+dense tensor that starts at a multiple of 16 bytes; empty ones are refused.  Every function launches on the current stream of
+its tensors' device.  There is no autograd behind them: the caller runs the backward pass, as `Trainer` does.
 """
 import ctypes as C
 
