@@ -549,9 +549,9 @@ int miseg_bn_bwd_sums(const double* stats, int32_t replicas, int32_t stride, int
  *
  * Tensors: dtype MISEG_DT_BF16 (16 bits in format fmt) or MISEG_DT_F32; `*_pix` / `*_img` are the strides of a pixel and of
  * an image in elements, so a tensor can be a channel slice of a wider buffer; pointers and strides are multiples of 16
- * bytes, C of 8; N <= 65535, pixels < 2^29, C <= 65536, none of them 0.  y may be x itself or another channel range of x's buffer and overlaps it in no other way.  Statistics
- * and sums are in fp32 per thread and fp64 across threads, without atomics: equal calls give equal bits.  Results are
- * rounded once; what exceeds the range of fp16 becomes an infinity.
+ * bytes, C of 8; N <= 65535, pixels < 2^29, C <= 65536, none of them 0.  y may be x itself or another channel range of x's
+ * buffer and overlaps it in no other way.  Statistics and sums are in fp32 per thread and fp64 across threads, without
+ * atomics: equal calls give equal bits.  Results are rounded once; what exceeds the range of fp16 becomes an infinity.
  * workspace: miseg_group_norm_workspace() bytes (none for the smallest maps), 16-byte aligned, not cleared by anyone; calls
  * that overlap in time need one each.
  */
