@@ -118,14 +118,17 @@ __device__ __forceinline__ void column_sums(double2* out, double2* tree, const f
     __syncthreads();
   }
 }
-// group[g] = sum over its channels of chan
-__device__ __forceinline__ void group_sums(double2* group, const double2* chan, double2* waves, int groups, int width) {
+// group[g] = sum over its channels of chan, which holds `channels` from number `first` of group 0 on.
+__device__ __forceinline__ void group_sums(double2* group, const double2* chan, double2* waves, int groups, int width,
+                                           int first, int channels) {
+  auto from = [&](int g) { return g == 0 ? 0 : g * width - first; };
+  auto to = [&](int g) { return (g + 1) * width - first < channels ? (g + 1) * width - first : channels; };
   if (width <= 16) {
     for (int g = threadIdx.x; g < groups; g += kNormThreads) {
-      double2 sum = chan[g * width];
-      for (int e = 1; e < width; ++e) {
-        sum.x += chan[g * width + e].x;
-        sum.y += chan[g * width + e].y;
+      double2 sum = make_double2(0, 0);
+      for (int e = from(g); e < to(g); ++e) {
+        sum.x += chan[e].x;
+        sum.y += chan[e].y;
       }
       group[g] = sum;
     }
@@ -133,9 +136,9 @@ __device__ __forceinline__ void group_sums(double2* group, const double2* chan, 
     const Segments sg(kNormThreads, groups);
     double2 sum = make_double2(0, 0);
     if (sg.seg < groups)
-      for (int e = sg.t; e < width; e += sg.lanes) {
-        sum.x += chan[sg.seg * width + e].x;
-        sum.y += chan[sg.seg * width + e].y;
+      for (int e = from(sg.seg) + sg.t; e < to(sg.seg); e += sg.lanes) {
+        sum.x += chan[e].x;
+        sum.y += chan[e].y;
       }
     sum = sg.sum(sum, waves);
     if (sg.seg < groups && sg.t == 0) group[sg.seg] = sum;
@@ -226,7 +229,7 @@ __global__ __launch_bounds__(kNormThreads) void gn_stats_kernel(const char* x, l
   const int c0 = blockIdx.y * wide, entries = (C - c0 < wide ? C - c0 : wide) / join;
   const double2* from = chan;
   if (join > 1) {
-    group_sums(group, chan, waves, entries, join);
+    group_sums(group, chan, waves, entries, join, 0, entries * join);
     from = group;
   }
   const double values = (double)(w.p1 - w.p0) * join;
@@ -238,7 +241,7 @@ __global__ __launch_bounds__(kNormThreads) void gn_stats_kernel(const char* x, l
 }
 
 // Sum over the threads of a block, in every thread.
-template <int TB> __device__ __forceinline__ double block_sum(double v, double* lds) {
+__device__ __forceinline__ double block_sum(double v, double* lds) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
   __syncthreads();
@@ -246,7 +249,7 @@ template <int TB> __device__ __forceinline__ double block_sum(double v, double* 
   __syncthreads();
   v = lds[0];
 #pragma unroll
-  for (int i = 1; i < TB / 64; ++i) v += lds[i];
+  for (int i = 1; i < kNormThreads / 64; ++i) v += lds[i];
   return v;
 }
 
@@ -281,8 +284,8 @@ __global__ __launch_bounds__(kNormThreads) void gn_finalize_kernel(const float2*
       q += (double)v[u].y + n * m * m;
     }
   }
-  s = block_sum<kNormThreads>(s, lds);
-  q = block_sum<kNormThreads>(q, lds);
+  s = block_sum(s, lds);
+  q = block_sum(q, lds);
   const double count = (double)pixels * w, m = s / count;
   double var = q / count - m * m;
   if (var < 0) var = 0;
@@ -565,7 +568,18 @@ __device__ __forceinline__ void bwd_coef(float (&za)[8], float (&zb)[8], const B
   }
 }
 
-// First pass: per block and channel sum g and sum g xhat; with `gpart` (one slab) also per group, times the channels' a.
+// The groups' partial sums of a slab, which may cut a group at either end: `pitch` entries, of the groups from first() on.
+struct GroupCuts {
+  int slab, width, pitch;
+  __device__ __forceinline__ GroupCuts(const NormGrid& g, int C, int width) : slab(g.cw * 8), width(width) {
+    const int most = (slab + width - 2) / width + 1, groups = C / width;
+    pitch = g.ny == 1 || most > groups ? groups : most;
+  }
+  __device__ __forceinline__ int first(int y) const { return y * slab / width; }
+};
+
+constexpr int kParamChannels = 16;                 // of a block that adds up partial sums by channels
+// First pass: per block and channel sum g and sum g xhat; with `gpart` also per group, times the channels' a.
 // XNT: x does not stay in the caches, as it and dy together are more than they hold.  Bound by reading: 157 MB (two images of
 // 480 x 640 x 64, x and dy) in 30 us, 241 MB (codes and dy of 960 x 1280 x 64) in 41 us (5.9 TB/s).
 template <typename T, int ACT, bool CK, bool XNT>
@@ -647,27 +661,41 @@ __global__ __launch_bounds__(kNormThreads) void gn_bwd_reduce_kernel(BwdArgs p, 
       part[((long long)w.n * gridDim.x + blockIdx.x) * p.C + c] = make_float2((float)a, (float)b);
       if (gpart) {
         const double sc = p.a[(long long)w.n * p.C + c];
-        chan[c] = make_double2(sc * a, sc * b);
+        chan[i] = make_double2(sc * a, sc * b);
       }
     }
   }
   if (gpart) {
+    const GroupCuts cuts(p.g, p.C, p.C / p.groups);
+    const int lo = blockIdx.y * wide, hi = lo + wide < p.C ? lo + wide : p.C, g0 = cuts.first(blockIdx.y);
+    const int groups = (hi - 1) / cuts.width - g0 + 1;
     __syncthreads();
-    group_sums(group, chan, waves, p.groups, p.C / p.groups);
-    for (int g = threadIdx.x; g < p.groups; g += kNormThreads)
-      gpart[((long long)w.n * gridDim.x + blockIdx.x) * p.groups + g] = make_float2((float)group[g].x, (float)group[g].y);
+    group_sums(group, chan, waves, groups, cuts.width, lo - g0 * cuts.width, hi - lo);
+    for (int g = threadIdx.x; g < groups; g += kNormThreads)
+      gpart[(((long long)w.n * gridDim.x + blockIdx.x) * p.g.ny + blockIdx.y) * cuts.pitch + g] =
+          make_float2((float)group[g].x, (float)group[g].y);
   }
 }
 
-// One block per (group, image): the channels' sums over the blocks, then over the group, in 64 bits.  Latency: 5 us.
-template <int TB>
-__global__ __launch_bounds__(TB) void gn_bwd_finalize_kernel(BwdArgs p, const float2* __restrict__ part, int blocks,
-                                                              int ckpt, double2* __restrict__ sums,
-                                                              float* __restrict__ cm, float* __restrict__ cz,
-                                                              float* __restrict__ cp, float* __restrict__ cq) {
-  __shared__ double r1[TB], r2[TB], lds[TB / 64];
+// Coefficients of the second pass from the group's mean g a (k1) and mean g a xhat (k2).
+__device__ __forceinline__ void bwd_share(const BwdArgs& p, int n, int c, double k1, double k2, float m, float rs, int ckpt,
+                                          float* cm, float* cz, float* cp, float* cq) {
+  const long long at = (long long)n * p.C + c;
+  cm[at] = !ckpt ? m : p.gamma ? p.gamma[c] : 1.f;
+  if (ckpt) cz[at] = p.beta ? p.beta[c] : 0.f;
+  cp[at] = (float)(ckpt ? -k2 : -k2 * rs);
+  cq[at] = (float)-k1;
+}
+
+// One block per (group, image): the channels' sums over the blocks, then over the group, in 64 bits.  Latency: 5 us, 7 from 8192
+// partial sums a group on.
+__global__ __launch_bounds__(kNormThreads) void gn_bwd_finalize_kernel(BwdArgs p, const float2* __restrict__ part, int blocks,
+                                                                      int ckpt, double2* __restrict__ sums,
+                                                                      float* __restrict__ cm, float* __restrict__ cz,
+                                                                      float* __restrict__ cp, float* __restrict__ cq) {
+  __shared__ double r1[kNormThreads], r2[kNormThreads], lds[kNormThreads / 64];
   const int w = p.C / p.groups, g = blockIdx.x, n = blockIdx.y;
-  const int wide = w < TB ? w : TB, lanes = TB / wide;
+  const int wide = w < kNormThreads ? w : kNormThreads, lanes = kNormThreads / wide;
   const int ci = threadIdx.x % wide, li = threadIdx.x / wide;
   double k1 = 0, k2 = 0;
   for (int c0 = 0; c0 < w; c0 += wide) {
@@ -701,16 +729,43 @@ __global__ __launch_bounds__(TB) void gn_bwd_finalize_kernel(BwdArgs p, const fl
     __syncthreads();
   }
   const double count = (double)p.pixels * w;
-  k1 = block_sum<TB>(k1, lds) / count;
-  k2 = block_sum<TB>(k2, lds) / count;
+  k1 = block_sum(k1, lds) / count;
+  k2 = block_sum(k2, lds) / count;
   const float m = p.mean[(long long)n * p.groups + g], rs = p.rstd[(long long)n * p.groups + g];
-  for (int i = threadIdx.x; i < w; i += TB) {
-    const int c = g * w + i;
-    const long long at = (long long)n * p.C + c;
-    cm[at] = !ckpt ? m : p.gamma ? p.gamma[c] : 1.f;
-    if (ckpt) cz[at] = p.beta ? p.beta[c] : 0.f;
-    cp[at] = (float)(ckpt ? -k2 : -k2 * rs);
-    cq[at] = (float)-k1;
+  for (int i = threadIdx.x; i < w; i += kNormThreads) bwd_share(p, n, g * w + i, k1, k2, m, rs, ckpt, cm, cz, cp, cq);
+}
+
+// The same where a group has more than 16384 partial sums, from the groups' partials of the blocks, by 16 channels of an image:
+// one group of 464 channels out of 127 blocks 9 us and 3 in the first pass, 21 in one block of 1024 threads; of 1536
+// channels out of 83 blocks 8 us, 38.
+__global__ __launch_bounds__(kNormThreads) void gn_bwd_finalize_wide_kernel(BwdArgs p, const float2* __restrict__ part,
+                                                                           int blocks, int ckpt, double2* __restrict__ sums,
+                                                                           float* __restrict__ cm, float* __restrict__ cz,
+                                                                           float* __restrict__ cp, float* __restrict__ cq) {
+  __shared__ double2 chan[kParamChannels], tree[kNormThreads];
+  __shared__ double lds[kNormThreads / 64];
+  const int c0 = blockIdx.x * kParamChannels, n = blockIdx.y;
+  const int channels = p.C - c0 < kParamChannels ? p.C - c0 : kParamChannels;
+  const GroupCuts cuts(p.g, p.C, p.C / p.groups);
+  column_sums(chan, tree, part + (long long)n * blocks * p.C + c0, blocks, channels, p.C,
+              [](int, float2 v) { return make_double2(v.x, v.y); });
+  if ((int)threadIdx.x < channels) sums[(long long)n * p.C + c0 + threadIdx.x] = chan[threadIdx.x];
+  const double count = (double)p.pixels * cuts.width;
+  const float2* gpart = p.gpart + (long long)n * blocks * p.g.ny * cuts.pitch;
+  for (int g = c0 / cuts.width; g * cuts.width < c0 + channels; ++g) {
+    const int y0 = g * cuts.width / cuts.slab, ys = ((g + 1) * cuts.width - 1) / cuts.slab - y0 + 1;
+    const float m = p.mean[(long long)n * p.groups + g], rs = p.rstd[(long long)n * p.groups + g];
+    double k1 = 0, k2 = 0;
+    for (int e = threadIdx.x; e < blocks * ys; e += kNormThreads) {
+      const int y = y0 + e % ys;
+      const float2 v = gpart[((long long)(e / ys) * p.g.ny + y) * cuts.pitch + g - cuts.first(y)];
+      k1 += v.x;
+      k2 += v.y;
+    }
+    k1 = block_sum(k1, lds) / count;
+    k2 = block_sum(k2, lds) / count;
+    const int c = c0 + threadIdx.x;
+    if ((int)threadIdx.x < channels && c / cuts.width == g) bwd_share(p, n, c, k1, k2, m, rs, ckpt, cm, cz, cp, cq);
   }
 }
 
@@ -790,7 +845,6 @@ __device__ __forceinline__ void bwd_apply(const BwdArgs& p, const NormWalk& w, c
   }
 }
 
-constexpr int kParamChannels = 16;                 // of a block that adds up the parameters' gradients
 // Second pass: dx = a g + (x - cm) cp + cq.  With dgamma or dbeta due, the blocks past the last pixels add them up.
 // FIN: every block adds up the groups' sums of its image for itself, which saves a launch.
 // Bound by memory: 157 MB out of the memory-side cache and 79 MB out in 34 us (6.9 TB/s); 84 MB of codes from HBM, 157 MB of
@@ -1251,6 +1305,9 @@ static SmallGrid small_grid(long long N, long long pixels, int C, int groups, bo
   return g;
 }
 
+// Partial sums of a group that one block adds up (10 thousand: 7 us, as the chip); more are left to the whole chip.
+constexpr int kWidePartials = 16384;
+
 static int images_per_step(long long N, long long image_bytes) {
   const long long n = kCacheBytes / image_bytes;
   return (int)(n < 1 ? 1 : n < N ? n : N);
@@ -1295,8 +1352,8 @@ static long long gn_workspace(long long N, long long pixels, int C, int groups, 
   const long long part = gn_partials(N, pixels, C), coef = round_up(4LL * N * C), sums = 2 * round_up(8LL * N * C);
   if (!backward) return small_fwd(N, pixels, C, groups, dtype, checkpoint).threads ? 0 : part + (checkpoint ? 2 * coef : 0);
   if (small_bwd(N, pixels, C, groups, dtype).threads) return N > 1 ? sums : 0;
-  // the coefficients, or, where the second pass works them out for itself, the groups' partial sums (at most the channels')
-  return sums + part + (part > 4 * coef ? part : 4 * coef);
+  return sums + part + 4 * coef + part;            // the groups' partial sums are at most as many as the channels'
+
 }
 
 static void launch_pass(const PassArgs& p, int N, int storage, int act, hipStream_t s) {
@@ -1460,7 +1517,7 @@ int launch_group_norm_bwd(const miseg_group_norm_bwd_desc* d, hipStream_t s) {
   const long long dbytes = d->pixels * d->C * bytes, xbytes = ck ? d->pixels * (d->C + 2 * ((d->C + 31) / 32)) : dbytes;
   // both stay in the cache if they can; else dy alone; else the last pixels of both
   const bool alone = xbytes + dbytes > kCacheBytes && dbytes <= kCacheBytes;
-  float2* gpart = fin ? (float2*)cm : nullptr;     // the coefficients' place: there are none in memory then
+  float2* gspace = (float2*)(ws + 4 * coef);
   const int step = fin ? d->N : images_per_step(d->N, alone ? dbytes : xbytes + dbytes);
   for (int n0 = 0; n0 < d->N; n0 += step) {
     const int n = d->N - n0 < step ? d->N - n0 : step;
@@ -1469,12 +1526,14 @@ int launch_group_norm_bwd(const miseg_group_norm_bwd_desc* d, hipStream_t s) {
               (char*)d->dx + n0 * d->dx_img * bytes, (const signed char*)d->codes, (const bf16_t*)d->code_scales,
               d->mean + gat, d->rstd + gat, d->scale + cat, d->shift + cat, d->gamma, d->beta, cm, cz, cp, cq, nullptr,
               d->dgamma, d->dbeta, d->x_pix, d->x_img, d->dy_pix, d->dy_img, d->dx_pix, d->dx_img, (int)d->pixels, d->C,
-              d->groups, d->N, fin ? few : norm_grid(n, d->pixels, d->C, kStatBlocks, kStatLeast), part, gpart, few.blocks};
+              d->groups, d->N, fin ? few : norm_grid(n, d->pixels, d->C, kStatBlocks, kStatLeast), part, gspace, few.blocks};
     if (ck) {
       p.codes += n0 * d->pixels * d->C;
       p.scales += n0 * d->pixels * ((d->C + 31) / 32);
     }
     const int blocks = p.g.blocks;
+    const bool wide = !fin && (long long)blocks * (d->C / d->groups) > kWidePartials;
+    float2* gpart = fin || wide ? gspace : nullptr;
     by_type_act(storage, act, [&](auto t, auto a) {
       typedef decltype(t) T;
       constexpr int A = decltype(a)::act;
@@ -1484,12 +1543,11 @@ int launch_group_norm_bwd(const miseg_group_norm_bwd_desc* d, hipStream_t s) {
       else if (alone) hipLaunchKernelGGL((gn_bwd_reduce_kernel<T, A, false, true>), grid, block, 0, s, p, part, gpart);
       else hipLaunchKernelGGL((gn_bwd_reduce_kernel<T, A, false, false>), grid, block, 0, s, p, part, gpart);
     });
-    // 1024 threads where a group has many partials: 8 x 60 x 582 x 312 in 4 groups 10 us with 256
-    if (!fin && (long long)blocks * (d->C / d->groups) > 4096)
-      hipLaunchKernelGGL((gn_bwd_finalize_kernel<1024>), dim3(d->groups, n), dim3(1024), 0, s, p, part, blocks, ck ? 1 : 0,
-                         sums + cat, cm, cz, cp, cq);
+    if (wide)
+      hipLaunchKernelGGL(gn_bwd_finalize_wide_kernel, dim3((d->C + kParamChannels - 1) / kParamChannels, n), dim3(kNormThreads),
+                         0, s, p, part, blocks, ck ? 1 : 0, sums + cat, cm, cz, cp, cq);
     else if (!fin)
-      hipLaunchKernelGGL((gn_bwd_finalize_kernel<256>), dim3(d->groups, n), dim3(256), 0, s, p, part, blocks, ck ? 1 : 0,
+      hipLaunchKernelGGL(gn_bwd_finalize_kernel, dim3(d->groups, n), dim3(kNormThreads), 0, s, p, part, blocks, ck ? 1 : 0,
                          sums + cat, cm, cz, cp, cq);
     p.g = norm_grid(n, d->pixels, d->C, fin ? kFewPass : kPassBlocks, kPassLeast);
     const bool params = n0 + n == d->N && (d->dgamma || d->dbeta);

@@ -221,6 +221,33 @@ def test_large_maps(ops, shape, checkpoint):
     close(dbeta, sums[1], sums[3])
 
 
+# groups of so many channels that the chip rather than a block adds up their partial sums; slabs that cut a group at one end, at
+# both ends, in the middle
+@pytest.mark.parametrize("shape,dt", [((3, 190, 200, 464, 1), torch.float32), ((2, 200, 210, 448, 2), torch.float32),
+                                      ((1, 75, 80, 1536, 1), torch.bfloat16), ((2, 75, 80, 1560, 3), torch.float16),
+                                      ((2, 64, 70, 1536, 6), torch.bfloat16), ((1, 90, 90, 2056, 1), torch.float32),
+                                      ((1, 90, 90, 4104, 27), torch.bfloat16)], ids=str)
+@pytest.mark.parametrize("checkpoint", [False, True])
+def test_groups_of_many_channels(ops, shape, dt, checkpoint):
+    n, h, w, c, groups = shape
+    act = "silu"
+    x, dy, gamma, beta = make(n, h, w, c, dt, seed=c + groups)
+    y, saved = ops.group_norm_act(x, gamma, beta, groups, act=act, checkpoint=checkpoint)
+    check_forward(x, y, saved, gamma, beta, groups, 1e-3, act)
+    dx, dgamma, dbeta = ops.group_norm_act_backward(dy, saved)
+    if checkpoint:
+        xhat = values(saved.checkpoint)
+        z, zmag = xhat * gamma.double() + beta.double(), (xhat * gamma.double()).abs() + beta.double().abs()
+    else:
+        scale, shift = saved.scale.double()[:, None, None], saved.shift.double()[:, None, None]
+        xhat = (x.double() - spread(saved.mean.double(), c)) * spread(saved.rstd.double(), c)
+        z, zmag = x.double() * scale + shift, (x.double() * scale).abs() + shift.abs()
+    wdx, wg, wb, tx, tg, tb = backward64(xhat, z, zmag, dy, saved.scale.double(), groups, act, dt)
+    close(dx, wdx, tx)
+    close(dgamma, wg, tg)
+    close(dbeta, wb, tb)
+
+
 def test_parameters_may_be_missing(ops):
     x, dy, gamma, beta = make(2, 9, 11, 48, torch.bfloat16)
     ones, zeros = torch.ones_like(gamma), torch.zeros_like(beta)
