@@ -112,11 +112,14 @@ def _view(t, name, like=None):
     n, h, w, c = t.shape
     if t.numel() == 0:
         raise L.MisegError("%s is empty: %s" % (name, tuple(t.shape)))
+    if n > 65535 or c > 65536:                               # before the 32 bits of a descriptor cut them
+        raise L.MisegError("%s: %d images of %d channels (at most 65535 of 65536)" % (name, n, c))
     if t.is_contiguous():
         return c, h * w * c
     sn, sh, sw, sc = t.stride()
     pix = sw if w > 1 else sh if h > 1 else max(sw, c)
-    if (c > 1 and sc != 1) or (w > 1 and h > 1 and sh != w * pix) or pix < c or (n > 1 and sn < (h * w - 1) * pix + c):
+    if (c > 1 and sc != 1) or (w > 1 and h > 1 and sh != w * pix) or not c <= pix < 1 << 31 or \
+            (n > 1 and sn < (h * w - 1) * pix + c):
         raise L.MisegError("%s is not channels last: shape %s, strides %s" % (name, tuple(t.shape), t.stride()))
     if h == 1 and w == 1:
         per = 16 // t.element_size()

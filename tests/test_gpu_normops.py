@@ -736,3 +736,19 @@ def test_most_pixels(ops):
         want = a * m - k1 - v * k2
         # k1 and k2 are known to the bound of the sums over the count
         close(dx[:, s], want, half_step(dx.dtype) * want.abs() + 8 * U * a.abs().max() * (8 + v.abs()))
+
+
+@pytest.mark.parametrize("shape,view", [((1, 1, 2, 2 ** 32 + 8), lambda t: t[..., :8]), ((1, 1, 1, 2 ** 32 + 8), lambda t: t),
+                                        ((2 ** 16, 1, 1, 8), lambda t: t), ((1, 1, 1, 65544), lambda t: t)],
+                         ids=["pixel stride", "channels cut", "images", "channels"])
+def test_extents_past_those_of_a_descriptor_are_refused(ops, shape, view):
+    from miseg_amd import lib as L
+    x = view(torch.empty(shape, dtype=torch.bfloat16, device="cuda"))
+    n, h, w, c = x.shape
+    flat = torch.zeros(1, device="cuda")
+    with pytest.raises(L.MisegError):
+        ops.group_norm_act(x, None, None, 1, checkpoint=True, out=x)
+    with pytest.raises(L.MisegError):
+        ops.checkpoint8_write(x)
+    with pytest.raises(L.MisegError):
+        ops.group_norm_act_backward(x, ops.Saved(x, None, flat, flat, flat, flat, None, None, 1, "none"))
