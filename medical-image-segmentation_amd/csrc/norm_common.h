@@ -114,7 +114,8 @@ struct NormGrid {
   int chunk, blocks;                               // pixels per block (a multiple of rows), blocks per image
 };
 
-// Blocks enough to fill the chip (`want` in all), none with less than `least` sweeps unless there are few of them anyway.
+// Blocks enough to fill the chip (`want` in all and no more, or the last ones run alone: 197 MB of statistics 35 us with 504
+// blocks, 42 with 516, when 512 are two a CU), none with less than `least` sweeps unless there are few of them anyway.
 static inline NormGrid norm_grid(long long N, long long pixels, int C, int want, int least, bool whole32 = false) {
   NormGrid g;
   const int unit = whole32 ? 4 : 1, c8 = (C / 8 + unit - 1) / unit * unit;
@@ -123,8 +124,9 @@ static inline NormGrid norm_grid(long long N, long long pixels, int C, int want,
   g.rows = kNormThreads / g.cw;
   const long long sweeps = (pixels + g.rows - 1) / g.rows, all = sweeps * N * g.ny;
   if (all < (long long)least * 1024) least = (int)(all / 1024) + 1;
-  long long b = (want + N * g.ny - 1) / (N * g.ny);
+  long long b = want / (N * g.ny);
   const long long most = (sweeps + least - 1) / least;
+  if (b < 1) b = 1;
   if (b > most) b = most;
   long long chunk = (pixels + b - 1) / b;
   chunk = (chunk + g.rows - 1) / g.rows * g.rows;

@@ -1330,12 +1330,12 @@ static bool few_partials(long long N, long long pixels, int C, int groups, int b
 
 static long long round_up(long long v) { return (v + 255) / 256 * 256; }
 
-// The blocks' partial sums, for steps of any number of images: norm_grid gives at most max(want, images x slabs) + images x
-// slabs - 1 blocks over all slabs, and a block writes cw * 8 channels at most.
+// The blocks' partial sums, for steps of any number of images: norm_grid gives at most max(want, images x slabs) blocks over
+// all slabs, and a block writes cw * 8 channels at most.
 static long long gn_partials(long long N, long long pixels, int C) {
   const NormGrid g = norm_grid(1, pixels, C, kStatBlocks, 1);
   const long long slab = 8LL * g.cw * 8, most = (long long)((pixels + g.rows - 1) / g.rows) * N * g.ny;
-  const long long blocks = kStatBlocks + 2 * N * g.ny;
+  const long long blocks = kStatBlocks + N * g.ny;
   return round_up(slab * (blocks < most ? blocks : most));
 }
 
