@@ -514,6 +514,43 @@ def test_captured_and_replayed(ops):
                 assert all(torch.equal(p, q) for p, q in zip(out, want))
 
 
+# the forms of three launches: steps of several images, groups that the chip adds up, slabs that cut groups
+@pytest.mark.parametrize("shape,dt", [((5, 480, 640, 64, 16), torch.bfloat16), ((3, 190, 200, 464, 1), torch.float32),
+                                      ((2, 75, 80, 1560, 3), torch.float16)], ids=str)
+def test_large_forms_on_two_streams_and_replayed(ops, shape, dt):
+    n, h, w, c, groups = shape
+    x, dy, gamma, beta = make(n, h, w, c, dt, seed=5)
+
+    def step():
+        y, s = ops.group_norm_act(x, gamma, beta, groups, act="silu", checkpoint=True)
+        y2, s2 = ops.group_norm_act(x, gamma, beta, groups, act="relu")
+        return (y, y2) + tuple(ops.group_norm_act_backward(dy, s)) + tuple(ops.group_norm_act_backward(dy, s2))
+    want = step()
+    torch.cuda.synchronize()
+    streams, results = [torch.cuda.Stream() for _ in range(2)], []
+    for i in range(4):
+        with torch.cuda.stream(streams[i % 2]):
+            results.append(step())
+    torch.cuda.synchronize()
+    for r in results:
+        assert all(torch.equal(p, q) for p, q in zip(r, want))
+    del results
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in (6, 7):
+        nx, ndy, _, _ = make(n, h, w, c, dt, seed=seed)
+        x.copy_(nx)
+        dy.copy_(ndy)
+        want = step()
+        for t in out:
+            t.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        step()
+        assert all(torch.equal(p, q) for p, q in zip(out, want))
+
+
 def test_offsets_past_32_bits(ops):
     """Channel slices of a 9 GB tensor: the second image starts 2^32 bytes in, rows of it lie past 2^31 elements."""
     c, wide = 32, 2048
