@@ -147,15 +147,36 @@ __device__ __forceinline__ void group_sums(double2* group, const double2* chan, 
 }
 constexpr int kSlabChannels = 512;                 // of norm_grid's widest slab
 
+// A block's partial sums a group, [image][block][slab][pitch]: a slab, which may cut a group at either end, holds those of the
+// groups from first() on, each over the channels of the group that lie in it.
+struct GroupCuts {
+  int slab, width, pitch, C;
+  __device__ __forceinline__ GroupCuts(const NormGrid& g, int C, int width) : slab(g.cw * 8), width(width), C(C) {
+    const int most = (slab + width - 2) / width + 1, groups = C / width;
+    pitch = g.ny == 1 || most > groups ? groups : most;
+  }
+  __device__ __forceinline__ int first(int y) const { return y * slab / width; }
+  __device__ __forceinline__ int end(int y) const { return (y + 1) * slab < C ? (y + 1) * slab : C; }
+  __device__ __forceinline__ int groups(int y) const { return (end(y) - 1) / width - first(y) + 1; }
+  __device__ __forceinline__ int channels(int g, int y) const {
+    const int from = g * width > y * slab ? g * width : y * slab, to = (g + 1) * width < end(y) ? (g + 1) * width : end(y);
+    return to - from;
+  }
+  // slabs that hold channels of group g
+  __device__ __forceinline__ int from_slab(int g) const { return g * width / slab; }
+  __device__ __forceinline__ int slabs(int g) const { return ((g + 1) * width - 1) / slab - from_slab(g) + 1; }
+};
+
 // ------------------------------------------------------------------------------------------------ forward statistics
 // Per block and channel: mean and sum of squared differences from it.  A thread sums (x - k) and (x - k)^2 with k its own
 // first value, so that an offset of the channel that is large against its spread does not cancel; threads and blocks are
-// joined by counts, means and sums of squares.  A partial holds `join` channels: a group where slabs hold whole groups, else 1.
+// joined by counts, means and sums of squares, a partial a group of the slab (a channel each where slabs cut groups: the
+// finalisation of 120 x 160 x 1536 in one group took 294 us, 6 so).
 // Bound by reading x: 157 MB in 30 us (5.3 TB/s).  512 blocks, two a CU, read as fast as 2048 and leave a quarter of the
 // partials: the finalisation of 960 x 1280 x 64 takes 4.9 us, 17 with 2048.
 template <typename T>
 __global__ __launch_bounds__(kNormThreads) void gn_stats_kernel(const char* x, long long xps, long long ximg, int pixels,
-                                                                int C, int join, NormGrid g, float2* __restrict__ part) {
+                                                                int C, int width, NormGrid g, float2* __restrict__ part) {
   constexpr int ES = Elem<T>::bytes, U = 4;
   __shared__ double2 chan[kSlabChannels], group[kSlabChannels], waves[kNormThreads / 64];
   __shared__ float lmean[kNormThreads * 8], lm2[kNormThreads * 8];
@@ -226,17 +247,17 @@ __global__ __launch_bounds__(kNormThreads) void gn_stats_kernel(const char* x, l
     if (q == 0 && i < wide) chan[i] = make_double2(sum, sq);
   }
   __syncthreads();
-  const int c0 = blockIdx.y * wide, entries = (C - c0 < wide ? C - c0 : wide) / join;
+  const GroupCuts cuts(g, C, width);
+  const int y = blockIdx.y, g0 = cuts.first(y), groups = cuts.groups(y);
   const double2* from = chan;
-  if (join > 1) {
-    group_sums(group, chan, waves, entries, join, 0, entries * join);
+  if (width > 1) {
+    group_sums(group, chan, waves, groups, width, y * wide - g0 * width, cuts.end(y) - y * wide);
     from = group;
   }
-  const double values = (double)(w.p1 - w.p0) * join;
-  for (int e = threadIdx.x; e < entries; e += kNormThreads) {
-    const double mean = from[e].x / values;
-    part[((long long)w.n * gridDim.x + blockIdx.x) * (C / join) + c0 / join + e] =
-        make_float2((float)mean, (float)(from[e].y - from[e].x * mean));
+  float2* out = part + (((long long)w.n * gridDim.x + blockIdx.x) * g.ny + y) * cuts.pitch;
+  for (int e = threadIdx.x; e < groups; e += kNormThreads) {
+    const double mean = from[e].x / ((double)(w.p1 - w.p0) * cuts.channels(g0 + e, y));
+    out[e] = make_float2((float)mean, (float)(from[e].y - from[e].x * mean));
   }
 }
 
@@ -254,8 +275,8 @@ __device__ __forceinline__ double block_sum(double v, double* lds) {
 }
 
 // One block per (group, image): the blocks' statistics of the group's channels in 64 bits, then the coefficients.
-__global__ __launch_bounds__(kNormThreads) void gn_finalize_kernel(const float2* __restrict__ part, int blocks, int chunk,
-                                                                   long long pixels, int C, int groups, int join,
+__global__ __launch_bounds__(kNormThreads) void gn_finalize_kernel(const float2* __restrict__ part, NormGrid grid,
+                                                                   long long pixels, int C, int groups,
                                                                    const float* __restrict__ gamma,
                                                                    const float* __restrict__ beta, float eps,
                                                                    float* __restrict__ mean, float* __restrict__ rstd,
@@ -264,24 +285,25 @@ __global__ __launch_bounds__(kNormThreads) void gn_finalize_kernel(const float2*
   __shared__ double lds[kNormThreads / 64];
   const int w = C / groups, g = blockIdx.x, n = blockIdx.y;
   double s = 0, q = 0;
-  const int each = w / join, pitch = C / join, entries = blocks * each;
-  const int last = (int)(pixels - (long long)(blocks - 1) * chunk);
-  const float2* pp = part + (long long)n * blocks * pitch + g * each;
+  const GroupCuts cuts(grid, C, w);
+  const int y0 = cuts.from_slab(g), ys = cuts.slabs(g), blocks = grid.blocks, entries = blocks * ys;
+  const int last = (int)(pixels - (long long)(blocks - 1) * grid.chunk);
+  const float2* pp = part + (long long)n * blocks * grid.ny * cuts.pitch + g;
   constexpr int U = 4;                             // loads in flight: the kernel waits for nothing else
   for (int e0 = threadIdx.x; e0 < entries; e0 += U * kNormThreads) {
     float2 v[U];
-    int count[U];
+    double count[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int e = e0 + u * kNormThreads, b = e / each;
-      count[u] = e >= entries ? 0 : b == blocks - 1 ? last : chunk;
-      v[u] = e < entries ? pp[(long long)b * pitch + (e - b * each)] : make_float2(0.f, 0.f);
+      const int e = e0 + u * kNormThreads, b = e / ys, y = y0 + e - b * ys;
+      count[u] = e >= entries ? 0. : (double)(b == blocks - 1 ? last : grid.chunk) * cuts.channels(g, y);
+      v[u] = e < entries ? pp[((long long)b * grid.ny + y) * cuts.pitch - cuts.first(y)] : make_float2(0.f, 0.f);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const double n = (double)count[u] * join, m = v[u].x;
-      s += n * m;
-      q += (double)v[u].y + n * m * m;
+      const double m = v[u].x;
+      s += count[u] * m;
+      q += (double)v[u].y + count[u] * m * m;
     }
   }
   s = block_sum(s, lds);
@@ -568,16 +590,6 @@ __device__ __forceinline__ void bwd_coef(float (&za)[8], float (&zb)[8], const B
   }
 }
 
-// The groups' partial sums of a slab, which may cut a group at either end: `pitch` entries, of the groups from first() on.
-struct GroupCuts {
-  int slab, width, pitch;
-  __device__ __forceinline__ GroupCuts(const NormGrid& g, int C, int width) : slab(g.cw * 8), width(width) {
-    const int most = (slab + width - 2) / width + 1, groups = C / width;
-    pitch = g.ny == 1 || most > groups ? groups : most;
-  }
-  __device__ __forceinline__ int first(int y) const { return y * slab / width; }
-};
-
 constexpr int kParamChannels = 16;                 // of a block that adds up partial sums by channels
 // First pass: per block and channel sum g and sum g xhat; with `gpart` also per group, times the channels' a.
 // XNT: x does not stay in the caches, as it and dy together are more than they hold.  Bound by reading: 157 MB (two images of
@@ -667,13 +679,11 @@ __global__ __launch_bounds__(kNormThreads) void gn_bwd_reduce_kernel(BwdArgs p, 
   }
   if (gpart) {
     const GroupCuts cuts(p.g, p.C, p.C / p.groups);
-    const int lo = blockIdx.y * wide, hi = lo + wide < p.C ? lo + wide : p.C, g0 = cuts.first(blockIdx.y);
-    const int groups = (hi - 1) / cuts.width - g0 + 1;
+    const int y = blockIdx.y, g0 = cuts.first(y), groups = cuts.groups(y);
     __syncthreads();
-    group_sums(group, chan, waves, groups, cuts.width, lo - g0 * cuts.width, hi - lo);
-    for (int g = threadIdx.x; g < groups; g += kNormThreads)
-      gpart[(((long long)w.n * gridDim.x + blockIdx.x) * p.g.ny + blockIdx.y) * cuts.pitch + g] =
-          make_float2((float)group[g].x, (float)group[g].y);
+    group_sums(group, chan, waves, groups, cuts.width, y * wide - g0 * cuts.width, cuts.end(y) - y * wide);
+    float2* out = gpart + (((long long)w.n * gridDim.x + blockIdx.x) * p.g.ny + y) * cuts.pitch;
+    for (int g = threadIdx.x; g < groups; g += kNormThreads) out[g] = make_float2((float)group[g].x, (float)group[g].y);
   }
 }
 
@@ -753,7 +763,7 @@ __global__ __launch_bounds__(kNormThreads) void gn_bwd_finalize_wide_kernel(BwdA
   const double count = (double)p.pixels * cuts.width;
   const float2* gpart = p.gpart + (long long)n * blocks * p.g.ny * cuts.pitch;
   for (int g = c0 / cuts.width; g * cuts.width < c0 + channels; ++g) {
-    const int y0 = g * cuts.width / cuts.slab, ys = ((g + 1) * cuts.width - 1) / cuts.slab - y0 + 1;
+    const int y0 = cuts.from_slab(g), ys = cuts.slabs(g);
     const float m = p.mean[(long long)n * p.groups + g], rs = p.rstd[(long long)n * p.groups + g];
     double k1 = 0, k2 = 0;
     for (int e = threadIdx.x; e < blocks * ys; e += kNormThreads) {
@@ -1436,14 +1446,13 @@ int launch_group_norm_fwd(const miseg_group_norm_desc* d, hipStream_t s) {
     const char* x = (const char*)d->x + n0 * d->x_img * bytes;
     const long long cat = (long long)n0 * d->C, gat = (long long)n0 * d->groups;
     const NormGrid g = norm_grid(n, d->pixels, d->C, kStatBlocks, kStatLeast);
-    const int width = d->C / d->groups, join = g.ny == 1 || g.cw * 8 % width == 0 ? width : 1;
     by_type_act(storage, NA_NONE, [&](auto t, auto) {
       hipLaunchKernelGGL((gn_stats_kernel<decltype(t)>), dim3(g.blocks, g.ny, n), dim3(kNormThreads), 0, s, x,
-                         (long long)d->x_pix, d->x_img, (int)d->pixels, d->C, join, g, part);
+                         (long long)d->x_pix, d->x_img, (int)d->pixels, d->C, d->C / d->groups, g, part);
     });
-    hipLaunchKernelGGL(gn_finalize_kernel, dim3(d->groups, n), dim3(kNormThreads), 0, s, part, g.blocks, g.chunk, d->pixels,
-                       d->C, d->groups, join, d->gamma, d->beta, d->eps, d->mean + gat, d->rstd + gat, d->scale + cat,
-                       d->shift + cat, qs, qt);
+    hipLaunchKernelGGL(gn_finalize_kernel, dim3(d->groups, n), dim3(kNormThreads), 0, s, part, g, d->pixels, d->C,
+                       d->groups, d->gamma, d->beta, d->eps, d->mean + gat, d->rstd + gat, d->scale + cat, d->shift + cat,
+                       qs, qt);
     PassArgs p{x, (char*)d->y + n0 * d->y_img * bytes, (signed char*)d->codes, (bf16_t*)d->code_scales, d->scale + cat,
                d->shift + cat, qs, qt, d->x_pix, d->x_img, d->y_pix, d->y_img, d->C, (int)d->pixels, d->C,
                norm_grid(n, d->pixels, d->C, kPassBlocks, kPassLeast, d->codes != nullptr)};
