@@ -80,8 +80,8 @@ __device__ __forceinline__ void unit_coef(float (&s)[8], float (&t)[8], const do
 
 // Per column the sums over `blocks` of f(block, partial) as out[c], C columns of partials in rows of `pitch`; 256 threads.
 // Loads are issued by fours: the partials were written by other chiplets, and a round trip takes about a microsecond.
-template <typename F>
-__device__ __forceinline__ void column_sums(double2* out, double2* tree, const float2* part, int blocks, int C, int pitch,
+template <typename V, typename F>
+__device__ __forceinline__ void column_sums(double2* out, double2* tree, const V* part, int blocks, int C, int pitch,
                                             F f) {
   constexpr int U = 4;
   const int wide = C < kNormThreads ? C : kNormThreads, parts = kNormThreads / wide;
@@ -91,10 +91,10 @@ __device__ __forceinline__ void column_sums(double2* out, double2* tree, const f
     double2 sum = make_double2(0, 0);
     if (share < parts && c < C)
       for (int k0 = share; k0 < blocks; k0 += U * parts) {
-        float2 v[U];
+        V v[U] = {};
 #pragma unroll
         for (int u = 0; u < U; ++u)
-          v[u] = k0 + u * parts < blocks ? part[(long long)(k0 + u * parts) * pitch + c] : make_float2(0.f, 0.f);
+          if (k0 + u * parts < blocks) v[u] = part[(long long)(k0 + u * parts) * pitch + c];
 #pragma unroll
         for (int u = 0; u < U; ++u)
           if (k0 + u * parts < blocks) {
@@ -1231,10 +1231,15 @@ __global__ __launch_bounds__(TB) void gn_small_bwd_kernel(SmallBwdArgs q) {
   else small_bwd_finish<T, NA_NONE, CK, V>(op, p.ops, v, a, za, zb, m, kp, kq, r, rows, p.pixels);
 }
 
+// The parameters' gradients by 16 channels.  Latency: 2 to 4 us; 3000 images of 16 channels 24 us, 100 with a thread a channel.
 __global__ __launch_bounds__(kNormThreads) void gn_bwd_params_kernel(const double2* __restrict__ sums, int images, int C,
                                                                      float* dgamma, float* dbeta) {
-  const int c = blockIdx.x * kNormThreads + threadIdx.x;
-  if (c < C) gn_bwd_params(sums, images, C, c, dgamma, dbeta);
+  __shared__ double2 chan[kParamChannels], tree[kNormThreads];
+  const int c0 = blockIdx.x * kParamChannels, channels = C - c0 < kParamChannels ? C - c0 : kParamChannels;
+  column_sums(chan, tree, sums + c0, images, channels, C, [](int, double2 v) { return v; });
+  if ((int)threadIdx.x >= channels) return;
+  if (dbeta) dbeta[c0 + threadIdx.x] = (float)chan[threadIdx.x].x;
+  if (dgamma) dgamma[c0 + threadIdx.x] = (float)chan[threadIdx.x].y;
 }
 
 // ------------------------------------------------------------------------------------------------ launches
@@ -1511,7 +1516,7 @@ int launch_group_norm_bwd(const miseg_group_norm_bwd_desc* d, hipStream_t s) {
       }
     });
     if (d->N > 1 && (d->dgamma || d->dbeta))
-      hipLaunchKernelGGL(gn_bwd_params_kernel, dim3((d->C + kNormThreads - 1) / kNormThreads), dim3(kNormThreads), 0, s, sums,
+      hipLaunchKernelGGL(gn_bwd_params_kernel, dim3((d->C + kParamChannels - 1) / kParamChannels), dim3(kNormThreads), 0, s, sums,
                          d->N, d->C, d->dgamma, d->dbeta);
     MISEG_CHECK_HIP(hipGetLastError());
     return MISEG_OK;
