@@ -226,10 +226,15 @@ static inline bool views_clash(const void* a, long long apix, long long aimg, co
   const char *pa = (const char*)a, *pb = (const char*)b;
   const long long ea = ((N - 1) * aimg + (pixels - 1) * apix + C) * bytes, eb = ((N - 1) * bimg + (pixels - 1) * bpix + C) * bytes;
   if (pa + ea <= pb || pb + eb <= pa) return false;
-  if (apix != bpix || (N > 1 && aimg != bimg)) return true;
+  if ((pixels > 1 && apix != bpix) || (N > 1 && aimg != bimg)) return true;
   if (pa == pb) return false;
-  long long d = pa < pb ? pb - pa : pa - pb;
-  if (N > 1 && aimg < pixels * apix) return true;
+  const long long d = pa < pb ? pb - pa : pa - pb;
+  if (pixels == 1) {                               // the pixel stride has no meaning: images lie where pixels do otherwise
+    if (N == 1) return true;
+    apix = aimg;
+  } else if (N > 1 && aimg < pixels * apix) {
+    return true;
+  }
   return d < (long long)C * bytes || d + (long long)C * bytes > apix * bytes;
 }
 

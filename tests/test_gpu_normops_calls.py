@@ -1,0 +1,58 @@
+"""Calls of the normalisation and checkpoint operators that their documentation allows, next to those of everyday use:
+slices of maps of one pixel, parameters that change before the backward pass, coefficients inside a flat buffer, arguments
+of other kinds, more blocks than one launch takes."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+@pytest.fixture(scope="module")
+def ops():
+    import miseg_amd  # noqa: F401
+    from miseg_amd import lib as L
+    from miseg_amd import normops
+    L.check(L.load().miseg_device_check())
+    return normops
+
+
+def normal(seed, *shape):
+    return torch.randn(shape, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda")
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=str)
+@pytest.mark.parametrize("n", [1, 4])
+def test_slices_of_maps_of_one_pixel(ops, dt, n):
+    """The pixel stride of a 1 x 1 map has no meaning: another channel range of the same buffer, reads and writes apart."""
+    buf = normal(1, n, 1, 1, 64).to(dt)
+    x, dst, gamma, beta = buf[..., :32], buf[..., 32:], normal(2, 32), normal(3, 32)
+    dy = normal(4, n, 1, 1, 32).to(dt)
+    keep = x.clone()
+    for ck in (False, True):
+        want, sw = ops.group_norm_act(keep, gamma, beta, 4, act="silu", checkpoint=ck)
+        y, s = ops.group_norm_act(x, gamma, beta, 4, act="silu", checkpoint=ck, out=dst)
+        assert torch.equal(y, want) and torch.equal(dst, want) and torch.equal(x, keep)
+        grads = ops.group_norm_act_backward(dy, sw)
+        dst.copy_(dy)
+        got = ops.group_norm_act_backward(dst, s, out=dst)
+        assert all(torch.equal(a, b) for a, b in zip(got, grads)) and torch.equal(x, keep)
+        if not ck:                                             # dx into the other half of x's buffer
+            got = ops.group_norm_act_backward(dy, s, out=dst)
+            assert all(torch.equal(a, b) for a, b in zip(got, grads)) and torch.equal(x, keep)
+    cw, yw = ops.checkpoint8_write(keep, None, None, gamma, beta, act="relu")
+    c, y = ops.checkpoint8_write(x, None, None, gamma, beta, act="relu", out=dst)
+    assert torch.equal(y, yw) and torch.equal(c.codes, cw.codes) and torch.equal(x, keep)
+
+
+def test_overlaps_of_maps_of_one_pixel_are_refused(ops):
+    from miseg_amd import lib as L
+    buf = normal(1, 3, 1, 1, 64).to(torch.bfloat16)
+    for out in (buf[..., 16:48], buf[..., 8:40]):
+        with pytest.raises(L.MisegError):
+            ops.group_norm_act(buf[..., :32], None, None, 4, out=out)
+    flat = normal(2, 128).to(torch.bfloat16)
+    with pytest.raises(L.MisegError):                          # the second image of x is the first of out
+        ops.group_norm_act(flat[:64].view(2, 1, 1, 32), None, None, 4, out=flat[32:96].view(2, 1, 1, 32))
