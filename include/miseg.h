@@ -574,6 +574,8 @@ typedef struct miseg_group_norm_desc {
   int32_t N, C, groups;
   int32_t dtype, fmt, act;
   float eps;
+  float* gamma_kept;           /* [C] each, 16-byte aligned, either may be NULL: gamma and beta as this call read them (1 and 0 */
+  float* beta_kept;            /* where there are none), for a backward pass from the checkpoint after they have changed */
 } miseg_group_norm_desc;
 int64_t miseg_group_norm_workspace(int32_t N, int64_t pixels, int32_t C, int32_t groups, int32_t dtype, int32_t checkpoint,
                                    int32_t backward);
@@ -584,7 +586,7 @@ int miseg_group_norm_act_fwd(const miseg_group_norm_desc* d, void* stream);
  *   g = dy * act'(z), z = x * scale + shift (checkpoint: xhat * gamma + beta)
  *   dbeta[c] = sum g;  dgamma[c] = sum g * xhat                                (either may be NULL)
  *   dx = scale * g - sum_group(scale * sum g) / m - xhat * sum_group(scale * sum g * xhat) / m
- * mean, rstd, scale, shift: of the forward call.  dx may be x or dy itself (or another channel range of their buffers).
+ * mean, rstd, scale, shift: of the forward call; gamma and beta: as the forward call read them.  dx may be x or dy itself (or another channel range of their buffers).
  */
 typedef struct miseg_group_norm_bwd_desc {
   const void* x;

@@ -168,6 +168,16 @@ __device__ __forceinline__ void store_coef(float* p, const float (&f)[8]) {
   *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
   *reinterpret_cast<float4*>(p + 4) = make_float4(f[4], f[5], f[6], f[7]);
 }
+// A layer's parameters, and where a call leaves what it read of them (or nowhere).
+struct NormParams {
+  const float *gamma, *beta;
+  float *gamma_kept, *beta_kept;
+  __device__ __forceinline__ void keep(int c) const {
+    float f[8];
+    if (gamma_kept) { load_param(f, gamma, c, 1.f); store_coef(gamma_kept + c, f); }
+    if (beta_kept) { load_param(f, beta, c, 0.f); store_coef(beta_kept + c, f); }
+  }
+};
 
 // ---- the 8-bit block format: 32 consecutive channels of a pixel share a bf16 scale, bf16(amax / 127).
 // code = rint(v / scale): |code| <= 127 because the scale's rounding moves amax / scale by at most 2^-9 of 127, less than

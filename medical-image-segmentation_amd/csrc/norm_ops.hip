@@ -276,9 +276,8 @@ __device__ __forceinline__ double block_sum(double v, double* lds) {
 
 // One block per (group, image): the blocks' statistics of the group's channels in 64 bits, then the coefficients.
 __global__ __launch_bounds__(kNormThreads) void gn_finalize_kernel(const float2* __restrict__ part, NormGrid grid,
-                                                                   long long pixels, int C, int groups,
-                                                                   const float* __restrict__ gamma,
-                                                                   const float* __restrict__ beta, float eps,
+                                                                   long long pixels, int C, int groups, NormParams param,
+                                                                   float eps,
                                                                    float* __restrict__ mean, float* __restrict__ rstd,
                                                                    float* __restrict__ scale, float* __restrict__ shift,
                                                                    float* __restrict__ qs, float* __restrict__ qt) {
@@ -318,9 +317,12 @@ __global__ __launch_bounds__(kNormThreads) void gn_finalize_kernel(const float2*
   }
   for (int i = threadIdx.x; i < w; i += kNormThreads) {
     const int c = g * w + i;
-    const double a = gamma ? gamma[c] * r : r;
+    const float gm = param.gamma ? param.gamma[c] : 1.f, bt = param.beta ? param.beta[c] : 0.f;
+    const double a = gm * r;
     scale[(long long)n * C + c] = (float)a;
-    shift[(long long)n * C + c] = (float)((beta ? beta[c] : 0.0) - m * a);
+    shift[(long long)n * C + c] = (float)(bt - m * a);
+    if (n == 0 && param.gamma_kept) param.gamma_kept[c] = gm;
+    if (n == 0 && param.beta_kept) param.beta_kept[c] = bt;
     if (qs) {
       qs[(long long)n * C + c] = (float)r;
       qt[(long long)n * C + c] = (float)(-m * r);
@@ -348,7 +350,7 @@ struct PassArgs {
   // FIN: group normalisation out of the partial statistics
   const float2* part = nullptr;
   int part_blocks = 0, part_chunk = 0, groups = 0;
-  const float *gamma = nullptr, *beta = nullptr;
+  NormParams param = {};
   float *mean = nullptr, *rstd = nullptr, *scale = nullptr, *shift = nullptr;
   float eps = 0.f;
 };
@@ -387,11 +389,12 @@ __global__ __launch_bounds__(kNormThreads) void norm_pass_kernel(PassArgs p) {
     __shared__ double2 group[kSlabChannels];
     pass_statistics(p, w.n, group);
     if (w.active) {
-      affine_coef(a, b, group, w.c, p.C / p.groups, p.gamma, p.beta, w.c);
+      affine_coef(a, b, group, w.c, p.C / p.groups, p.param.gamma, p.param.beta, w.c);
       if (Q) unit_coef(s, t, group, w.c, p.C / p.groups);
       if (blockIdx.x == 0 && w.r == 0) {
         store_coef(p.scale + (long long)w.n * p.C + w.c, a);
         store_coef(p.shift + (long long)w.n * p.C + w.c, b);
+        if (w.n == 0) p.param.keep(w.c);
       }
     }
   }
@@ -935,7 +938,7 @@ struct SmallFwdArgs {
   char* y;
   signed char* codes;
   bf16_t* scales;
-  const float *gamma, *beta;
+  NormParams param;
   float *mean, *rstd, *a, *b;
   long long xps, ximg, yps, yimg;
   int pixels, C, groups, act, blocks;
@@ -1051,10 +1054,11 @@ __global__ __launch_bounds__(TB) void gn_small_fwd_kernel(SmallFwdArgs p) {
   __syncthreads();
   if (active) {
     float a[8], b[8];
-    affine_coef(a, b, stat, l * 8, width, p.gamma, p.beta, c);
+    affine_coef(a, b, stat, l * 8, width, p.param.gamma, p.param.beta, c);
     if (r == 0) {
       store_coef(p.a + (long long)n * p.C + c, a);
       store_coef(p.b + (long long)n * p.C + c, b);
+      if (n == 0) p.param.keep(c);
     }
     char* yp = p.y + (n * p.yimg + c) * ES;
     if (p.act == NA_RELU) small_fwd_finish<T, NA_RELU, V>(yp, p.yps, v, a, b, r, rows, p.pixels);
@@ -1396,6 +1400,8 @@ int launch_group_norm_fwd(const miseg_group_norm_desc* d, hipStream_t s) {
                   "group_norm_act: y overlaps x without being x or another channel range of its buffer");
   MISEG_CHECK_ARG(d->mean && d->rstd && d->scale && d->shift && good_coef(d->scale) && good_coef(d->shift),
                   "group_norm_act: mean, rstd, scale and shift are needed, scale and shift 16-byte aligned");
+  MISEG_CHECK_ARG(good_coef(d->gamma_kept) && good_coef(d->beta_kept),
+                  "group_norm_act: gamma_kept and beta_kept must be 16-byte aligned");
   MISEG_CHECK_ARG(d->eps >= 0.f, "group_norm_act: eps = %g", (double)d->eps);
   MISEG_CHECK_ARG(!d->codes == !d->code_scales && ((uintptr_t)d->codes & 7) == 0 && ((uintptr_t)d->code_scales & 1) == 0,
                   "group_norm_act: codes and code_scales go together, 8-byte and 2-byte aligned");
@@ -1404,9 +1410,10 @@ int launch_group_norm_fwd(const miseg_group_norm_desc* d, hipStream_t s) {
                   "group_norm_act: the workspace must be 16-byte aligned and hold %lld bytes (%lld given)", need,
                   (long long)d->workspace_bytes);
   const int storage = storage_of(d->dtype, d->fmt);
+  const NormParams param{d->gamma, d->beta, d->gamma_kept, d->beta_kept};
   const SmallGrid sg = small_fwd(d->N, d->pixels, d->C, d->groups, d->dtype, d->codes != nullptr);
   if (sg.threads) {
-    SmallFwdArgs p{(const char*)d->x, (char*)d->y, (signed char*)d->codes, (bf16_t*)d->code_scales, d->gamma, d->beta,
+    SmallFwdArgs p{(const char*)d->x, (char*)d->y, (signed char*)d->codes, (bf16_t*)d->code_scales, param,
                    d->mean, d->rstd, d->scale, d->shift, d->x_pix, d->x_img, d->y_pix, d->y_img, (int)d->pixels, d->C,
                    d->groups, act_of(d->act), d->N * sg.slabs, d->eps, sg};
     const dim3 grid(p.blocks), block(sg.threads);
@@ -1440,7 +1447,7 @@ int launch_group_norm_fwd(const miseg_group_norm_desc* d, hipStream_t s) {
     PassArgs p{(const char*)d->x, (char*)d->y, (signed char*)d->codes, (bf16_t*)d->code_scales, nullptr, nullptr, nullptr,
                nullptr, d->x_pix, d->x_img, d->y_pix, d->y_img, d->C, (int)d->pixels, d->C,
                norm_grid(d->N, d->pixels, d->C, kFewPass, kPassLeast, d->codes != nullptr), part, g.blocks, g.chunk,
-               d->groups, d->gamma, d->beta, d->mean, d->rstd, d->scale, d->shift, d->eps};
+               d->groups, param, d->mean, d->rstd, d->scale, d->shift, d->eps};
     launch_pass(p, d->N, storage, act_of(d->act), s);
     MISEG_CHECK_HIP(hipGetLastError());
     return MISEG_OK;
@@ -1456,7 +1463,7 @@ int launch_group_norm_fwd(const miseg_group_norm_desc* d, hipStream_t s) {
                          (long long)d->x_pix, d->x_img, (int)d->pixels, d->C, d->C / d->groups, g, part);
     });
     hipLaunchKernelGGL(gn_finalize_kernel, dim3(d->groups, n), dim3(kNormThreads), 0, s, part, g, d->pixels, d->C,
-                       d->groups, d->gamma, d->beta, d->eps, d->mean + gat, d->rstd + gat, d->scale + cat, d->shift + cat,
+                       d->groups, n0 ? NormParams{d->gamma, d->beta, nullptr, nullptr} : param, d->eps, d->mean + gat, d->rstd + gat, d->scale + cat, d->shift + cat,
                        qs, qt);
     PassArgs p{x, (char*)d->y + n0 * d->y_img * bytes, (signed char*)d->codes, (bf16_t*)d->code_scales, d->scale + cat,
                d->shift + cat, qs, qt, d->x_pix, d->x_img, d->y_pix, d->y_img, d->C, (int)d->pixels, d->C,

@@ -116,6 +116,7 @@ class GroupNormDesc(C.Structure):
         ("workspace_bytes", C.c_int64), ("pixels", C.c_int64), ("x_img", C.c_int64), ("y_img", C.c_int64),
         ("x_pix", C.c_int32), ("y_pix", C.c_int32), ("N", C.c_int32), ("C", C.c_int32), ("groups", C.c_int32),
         ("dtype", C.c_int32), ("fmt", C.c_int32), ("act", C.c_int32), ("eps", C.c_float),
+        ("gamma_kept", C.c_void_p), ("beta_kept", C.c_void_p),
     ]
 
 

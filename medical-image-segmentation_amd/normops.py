@@ -55,7 +55,9 @@ class Checkpoint8:
 
 class Saved:
     """What `group_norm_act_backward` takes of a forward call: x or its checkpoint, the statistics `mean` and `rstd`
-    (N, groups), the coefficients of z = x * scale + shift (N, C), and the layer's parameters."""
+    (N, groups), the coefficients of z = x * scale + shift (N, C), and the layer's parameters `gamma` and `beta` (None
+    where it has none), which only the backward pass from a checkpoint reads: a forward call that writes one keeps them as
+    it read them, so that an update in between changes no gradient."""
 
     def __init__(self, x, checkpoint, mean, rstd, scale, shift, gamma, beta, groups, act):
         self.x, self.checkpoint = x, checkpoint
@@ -64,21 +66,35 @@ class Saved:
 
     @classmethod
     def _of(cls, x, checkpoint, flat, n, c, gamma, beta, groups, act):
-        """From the buffer of a forward call, scale, shift, mean, rstd one behind the other: taken apart where somebody asks."""
+        """From the buffer of a forward call, scale, shift, mean, rstd and with a checkpoint gamma and beta between shift and
+        mean, one behind the other: taken apart where somebody asks."""
         self = cls(x, checkpoint, None, None, None, None, gamma, beta, groups, act)
-        self._four, self._flat, self._n, self._c = None, flat, n, c
+        self._four, self._flat, self._n, self._c, self._stats = None, flat, n, c, 2 * n * c
+        if checkpoint is not None:
+            self._stats += 2 * c
+            if gamma is not None:
+                del self.gamma                               # __getattr__ finds it in the buffer
+            if beta is not None:
+                del self.beta
         return self
+
+    def __getattr__(self, name):
+        if name not in ("gamma", "beta"):
+            raise AttributeError(name)
+        t = self._flat.as_strided((self._c,), (1,), (2 * self._n + (name == "beta")) * self._c)
+        setattr(self, name, t)
+        return t
 
     def _part(self, which, columns, start):
         return self._four[which] if self._four else self._flat.as_strided((self._n, columns), (columns, 1), start)
 
     @property
     def mean(self):
-        return self._part(0, self.groups, 0 if self._four else 2 * self._n * self._c)
+        return self._part(0, self.groups, 0 if self._four else self._stats)
 
     @property
     def rstd(self):
-        return self._part(1, self.groups, 0 if self._four else self._n * (2 * self._c + self.groups))
+        return self._part(1, self.groups, 0 if self._four else self._stats + self._n * self.groups)
 
     @property
     def scale(self):
@@ -96,9 +112,17 @@ class Saved:
                 raise L.MisegError("saved from %d images of %d channels on %s, not %d of %d on %s"
                                    % (self._n, self._c, self._flat.device, n, c, device))
             at = self._flat.data_ptr()
-            return at + 8 * n * c, at + 4 * n * (2 * c + g), at, at + 4 * n * c
+            stats = at + 4 * self._stats
+            return stats, stats + 4 * n * g, at, at + 4 * n * c
         return tuple(_coef(t, name, shape, device, False) for t, name, shape in
                      zip(self._four, ("mean", "rstd", "scale", "shift"), ((n, g), (n, g), (n, c), (n, c))))
+
+    def _parameters(self, n, c, device):
+        """Addresses of gamma and beta, or None; after `_addresses`."""
+        own = self.__dict__
+        at = self._flat.data_ptr() + 8 * n * c if "gamma" not in own or "beta" not in own else 0
+        return _coef(self.gamma, "gamma", (c,), device) if "gamma" in own else at, \
+            _coef(self.beta, "beta", (c,), device) if "beta" in own else at + 4 * c
 
 
 def _view(t, name, like=None):
@@ -194,14 +218,20 @@ def group_norm_act(x, gamma, beta, groups, eps=1e-3, act="none", out=None, check
         if y.data_ptr() == d.x and not checkpoint:
             raise L.MisegError("out is x, which the backward pass needs: pass checkpoint=True or another tensor")
     d.y = y.data_ptr()
-    flat = x.new_empty(2 * n * (c + groups), dtype=torch.float32)
+    flat = x.new_empty(2 * (n * (c + groups) + (c if checkpoint else 0)), dtype=torch.float32)
     d.gamma, d.beta = _coef(gamma, "gamma", (c,), device), _coef(beta, "beta", (c,), device)
     d.scale = at = flat.data_ptr()
-    d.shift, d.mean, d.rstd = at + 4 * n * c, at + 8 * n * c, at + 4 * n * (2 * c + groups)
+    d.shift, stats = at + 4 * n * c, at + 8 * n * c
     ck = None
     if checkpoint:
+        if gamma is not None:
+            d.gamma_kept = stats
+        if beta is not None:
+            d.beta_kept = stats + 4 * c
+        stats += 8 * c
         ck = Checkpoint8._like(x)
         d.codes, d.code_scales = ck.codes.data_ptr(), ck.scales.data_ptr()
+    d.mean, d.rstd = stats, stats + 4 * n * groups
     d.N, d.C, d.groups, d.pixels, d.eps, d.act = n, c, groups, h * w, eps, _act(act)
     d.dtype, d.fmt = _TYPES[dtype]
     ws = _workspace(lib, d, 1 if checkpoint else 0, 0, x)    # noqa: F841: lives until the launch is in its stream
@@ -240,7 +270,7 @@ def group_norm_act_backward(dy, saved, out=None):
             raise L.MisegError("out is %s, dy %s" % (dx.dtype, dtype))
     d.dx = dx.data_ptr()
     d.mean, d.rstd, d.scale, d.shift = saved._addresses(n, c, device)
-    d.gamma, d.beta = _coef(saved.gamma, "gamma", (c,), device), _coef(saved.beta, "beta", (c,), device)
+    d.gamma, d.beta = saved._parameters(n, c, device)
     grads = dy.new_empty((2, c), dtype=torch.float32)
     d.dgamma = at = grads.data_ptr()
     d.dbeta = at + 4 * c

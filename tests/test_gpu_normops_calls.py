@@ -56,3 +56,26 @@ def test_overlaps_of_maps_of_one_pixel_are_refused(ops):
     flat = normal(2, 128).to(torch.bfloat16)
     with pytest.raises(L.MisegError):                          # the second image of x is the first of out
         ops.group_norm_act(flat[:64].view(2, 1, 1, 32), None, None, 4, out=flat[32:96].view(2, 1, 1, 32))
+
+
+# the form of one launch, of two, of three; one image and several
+@pytest.mark.parametrize("shape", [(1, 15, 20, 64, 8), (2, 9, 11, 72, 9), (2, 90, 80, 72, 9), (2, 30, 31, 520, 5), (9, 480, 640, 64, 16)], ids=str)
+def test_parameters_that_change_before_the_backward_pass(ops, shape):
+    """The backward pass is that of the forward call: what an optimiser does to gamma and beta in between is not seen."""
+    n, h, w, c, groups = shape
+    x, dy = normal(1, n, h, w, c).to(torch.bfloat16), normal(2, n, h, w, c).to(torch.bfloat16)
+    for ck in (False, True):
+        for which in ("both", "gamma", "beta"):
+            gamma = None if which == "beta" else normal(3, c)
+            beta = None if which == "gamma" else normal(4, c)
+            _, saved = ops.group_norm_act(x, gamma, beta, groups, act="relu", checkpoint=ck)
+            want = ops.group_norm_act_backward(dy, saved)
+            first = [None if t is None else t.clone() for t in (gamma, beta)]
+            for t in (gamma, beta):
+                if t is not None:
+                    t.neg_().add_(0.25)
+            got = ops.group_norm_act_backward(dy, saved)
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), (ck, which)
+            if ck:
+                for have, t in zip((saved.gamma, saved.beta), first):
+                    assert have is None and t is None or torch.equal(have, t)
