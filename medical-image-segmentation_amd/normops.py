@@ -6,7 +6,8 @@ batch statistics only): `group_norm_act` and `group_norm_act_backward` for batch
 
 Tensors are (N, H, W, C) with C a multiple of 8, in bfloat16, float16 or float32, dense or a channel slice of a wider
 dense tensor that starts at a multiple of 16 bytes; empty ones are refused.  Every function launches on the current stream of
-its tensors' device.  There is no autograd behind them: the caller runs the backward pass, as `Trainer` does.
+its tensors' device.  There is no autograd behind them: the caller runs the backward pass, as `Trainer` does.  Where autograd
+is recording, a tensor that asks for a gradient is refused: take `.detach()` of it or call under `torch.no_grad()`.
 """
 import ctypes as C
 
@@ -160,6 +161,14 @@ def _coef(t, name, shape, device, optional=True):
     return t.data_ptr()
 
 
+def _plain(*tensors):
+    """Nothing that autograd would have to see."""
+    for t in tensors:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise L.MisegError("a tensor asks for a gradient, and no autograd is behind this call: detach it or call under "
+                               "torch.no_grad()")
+
+
 def _act(act):
     if act not in ACTS:
         raise L.MisegError("activation %r: one of %s" % (act, ", ".join(ACTS)))
@@ -218,8 +227,9 @@ def group_norm_act(x, gamma, beta, groups, eps=1e-3, act="none", out=None, check
         if y.data_ptr() == d.x and not checkpoint:
             raise L.MisegError("out is x, which the backward pass needs: pass checkpoint=True or another tensor")
     d.y = y.data_ptr()
-    flat = x.new_empty(2 * (n * (c + groups) + (c if checkpoint else 0)), dtype=torch.float32)
     d.gamma, d.beta = _coef(gamma, "gamma", (c,), device), _coef(beta, "beta", (c,), device)
+    _plain(x, gamma, beta, out)
+    flat = x.new_empty(2 * (n * (c + groups) + (c if checkpoint else 0)), dtype=torch.float32)
     d.scale = at = flat.data_ptr()
     d.shift, stats = at + 4 * n * c, at + 8 * n * c
     ck = None
@@ -268,6 +278,7 @@ def group_norm_act_backward(dy, saved, out=None):
         d.dx_pix, d.dx_img = _view(dx, "out", dy)
         if dx.dtype != dtype:
             raise L.MisegError("out is %s, dy %s" % (dx.dtype, dtype))
+    _plain(dy, out)
     d.dx = dx.data_ptr()
     d.mean, d.rstd, d.scale, d.shift = saved._addresses(n, c, device)
     d.gamma, d.beta = saved._parameters(n, c, device)
@@ -315,6 +326,7 @@ def checkpoint8_write(x, scale=None, shift=None, y_scale=None, y_shift=None, act
         d.y = y.data_ptr()
     elif out is not None or act != "none":
         raise L.MisegError("an activation and out belong to y, which takes y_scale and y_shift")
+    _plain(x, scale, shift, y_scale, y_shift, out)
     ck = Checkpoint8._like(x)
     d.codes, d.code_scales = ck.codes.data_ptr(), ck.scales.data_ptr()
     d.N, d.C, d.pixels, d.act = n, c, h * w, _act(act)
@@ -335,6 +347,7 @@ def checkpoint8_read(checkpoint, scale=None, shift=None, act="none", dtype=torch
     d.y_pix, d.y_img = _view(out, "out", checkpoint)
     d.y, d.codes, d.code_scales = out.data_ptr(), codes.data_ptr(), checkpoint.scales.data_ptr()
     d.y_a, d.y_b, d.coef_img = _pair(scale, shift, "y", n, c, device)
+    _plain(scale, shift, out)
     d.N, d.C, d.pixels, d.act = n, c, h * w, _act(act)
     d.dtype, d.fmt = _TYPES[out.dtype]
     _launch(lib.miseg_checkpoint8_read, d, device)

@@ -79,3 +79,32 @@ def test_parameters_that_change_before_the_backward_pass(ops, shape):
             if ck:
                 for have, t in zip((saved.gamma, saved.beta), first):
                     assert have is None and t is None or torch.equal(have, t)
+
+
+def test_tensors_that_ask_for_a_gradient_are_refused(ops):
+    """No autograd behind these calls: a result without a gradient in place of one that was asked for would go unseen."""
+    from miseg_amd import lib as L
+    x, dy, gamma, beta = normal(1, 2, 5, 6, 32), normal(2, 2, 5, 6, 32), normal(3, 32), normal(4, 32)
+    y, saved = ops.group_norm_act(x, gamma, beta, 4, act="silu", checkpoint=True)
+    ck = saved.checkpoint
+
+    def calls(x, dy, gamma, beta):
+        return {"forward": lambda: ops.group_norm_act(x, gamma, beta, 4, act="silu", checkpoint=True)[0],
+                "backward": lambda: ops.group_norm_act_backward(dy, saved)[0],
+                "write": lambda: ops.checkpoint8_write(x, gamma, beta, gamma, beta)[1],
+                "read": lambda: ops.checkpoint8_read(ck, gamma, beta, dtype=torch.float32)}
+    takes = {"x": ("forward", "write"), "dy": ("backward",), "gamma": ("forward", "write", "read"), "beta": ("forward", "write", "read")}
+    plain = {k: f() for k, f in calls(x, dy, gamma, beta).items()}
+    for name, users in takes.items():
+        args = dict(x=x, dy=dy, gamma=gamma, beta=beta)
+        args[name] = args[name].clone().requires_grad_()
+        for user, f in calls(**args).items():
+            if user in users:
+                with pytest.raises(L.MisegError, match="gradient"):
+                    f()
+                with torch.no_grad():
+                    assert torch.equal(f(), plain[user])
+            else:
+                assert torch.equal(f(), plain[user])
+    with pytest.raises(L.MisegError, match="gradient"):
+        ops.group_norm_act(x, gamma, beta, 4, out=torch.empty_like(x, requires_grad=True))
