@@ -293,14 +293,26 @@ def group_norm_act_backward(dy, saved, out=None):
     return dx, dgamma, dbeta
 
 
+def _aligned(t):
+    """t, or a copy of it at a multiple of 16 bytes: a slice of a flat buffer need not start at one."""
+    return t if t.data_ptr() & 15 == 0 else t.clone()
+
+
 def _pair(a, b, what, n, c, device):
-    """Coefficients (C,) or (N, C) as (pointer, pointer, elements from one image's to the next's)."""
+    """Coefficients (C,) or (N, C) as (tensor, tensor, elements from one image's to the next's); the caller holds them until
+    the launch is in its stream."""
     if a is None and b is None:
         return None, None, 0
     if a is None or b is None:
         raise L.MisegError("%s: a scale and a shift go together" % what)
     shape = (n, c) if a.dim() == 2 else (c,)
-    return _coef(a, what + " scale", shape, device), _coef(b, what + " shift", shape, device), c if a.dim() == 2 else 0
+    _coef(a, what + " scale", shape, device)
+    _coef(b, what + " shift", shape, device)
+    return _aligned(a), _aligned(b), c if a.dim() == 2 else 0
+
+
+def _pointers(a, b):
+    return (None, None) if a is None else (a.data_ptr(), b.data_ptr())
 
 
 def checkpoint8_write(x, scale=None, shift=None, y_scale=None, y_shift=None, act="none", out=None):
@@ -312,8 +324,10 @@ def checkpoint8_write(x, scale=None, shift=None, y_scale=None, y_shift=None, act
     n, h, w, c = x.shape
     device = x.device
     d.x = x.data_ptr()
-    d.code_a, d.code_b, img = _pair(scale, shift, "code", n, c, device)
-    d.y_a, d.y_b, y_of = _pair(y_scale, y_shift, "y", n, c, device)
+    scale, shift, img = _pair(scale, shift, "code", n, c, device)
+    y_scale, y_shift, y_of = _pair(y_scale, y_shift, "y", n, c, device)
+    d.code_a, d.code_b = _pointers(scale, shift)
+    d.y_a, d.y_b = _pointers(y_scale, y_shift)
     if scale is not None and y_scale is not None and img != y_of:
         raise L.MisegError("the coefficients of the codes and of y are both (C,) or both (N, C)")
     d.coef_img = max(img, y_of)
@@ -346,7 +360,8 @@ def checkpoint8_read(checkpoint, scale=None, shift=None, act="none", dtype=torch
     d = L.Checkpoint8Desc()
     d.y_pix, d.y_img = _view(out, "out", checkpoint)
     d.y, d.codes, d.code_scales = out.data_ptr(), codes.data_ptr(), checkpoint.scales.data_ptr()
-    d.y_a, d.y_b, d.coef_img = _pair(scale, shift, "y", n, c, device)
+    scale, shift, d.coef_img = _pair(scale, shift, "y", n, c, device)
+    d.y_a, d.y_b = _pointers(scale, shift)
     _plain(scale, shift, out)
     d.N, d.C, d.pixels, d.act = n, c, h * w, _act(act)
     d.dtype, d.fmt = _TYPES[out.dtype]

@@ -108,3 +108,53 @@ def test_tensors_that_ask_for_a_gradient_are_refused(ops):
                 assert torch.equal(f(), plain[user])
     with pytest.raises(L.MisegError, match="gradient"):
         ops.group_norm_act(x, gamma, beta, 4, out=torch.empty_like(x, requires_grad=True))
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=str)
+@pytest.mark.parametrize("per_image", [False, True])
+def test_coefficients_inside_a_flat_buffer(ops, dt, per_image):
+    """Slices at odd offsets, as group_norm_act takes them, in the calls that go with it."""
+    n, h, w, c = 2, 7, 9, 40
+    x = normal(1, n, h, w, c).to(dt)
+    count = n * c if per_image else c
+    flat = normal(2, 4 * count + 8)
+    odd = [flat[i * (count + 1) + 1:][:count] for i in range(4)]
+    if per_image:
+        odd = [t.view(n, c) for t in odd]
+    assert any(t.data_ptr() % 16 for t in odd)
+    even = [t.clone() for t in odd]
+    ck, y = ops.checkpoint8_write(x, *odd, act="silu")
+    cw, yw = ops.checkpoint8_write(x, *even, act="silu")
+    assert torch.equal(y, yw) and torch.equal(ck.codes, cw.codes) and torch.equal(ck.scales, cw.scales)
+    got = ops.checkpoint8_read(ck, odd[0], odd[1], act="relu", dtype=dt)
+    assert torch.equal(got, ops.checkpoint8_read(ck, even[0], even[1], act="relu", dtype=dt))
+    if not per_image:
+        gamma, beta = odd[0], odd[1]
+        _, saved = ops.group_norm_act(x, gamma, beta, 5, act="relu", checkpoint=True)
+        got = ops.checkpoint8_read(saved.checkpoint, gamma, beta, act="relu", dtype=dt)
+        assert torch.equal(got, ops.checkpoint8_read(saved.checkpoint, even[0], even[1], act="relu", dtype=dt))
+
+
+def test_coefficients_inside_a_flat_buffer_captured(ops):
+    x, flat = normal(1, 2, 7, 9, 40).to(torch.bfloat16), normal(2, 83)
+    gamma, beta = flat[1:41], flat[42:82]
+
+    def step():
+        ck, y = ops.checkpoint8_write(x, gamma, beta, gamma, beta, act="relu")
+        return y, ck.codes, ops.checkpoint8_read(ck, gamma, beta, act="relu")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in (3, 4, 5):
+        x.copy_(normal(seed, 2, 7, 9, 40))
+        flat.copy_(normal(seed + 10, 83))
+        want = step()
+        out[0].fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
