@@ -308,7 +308,7 @@ def _pair(a, b, what, n, c, device):
     shape = (n, c) if a.dim() == 2 else (c,)
     _coef(a, what + " scale", shape, device)
     _coef(b, what + " shift", shape, device)
-    return _aligned(a), _aligned(b), c if a.dim() == 2 else 0
+    return _aligned(a), _aligned(b), c if a.dim() == 2 and n > 1 else 0      # of one image both shapes are the same
 
 
 def _pointers(a, b):

@@ -158,3 +158,14 @@ def test_coefficients_inside_a_flat_buffer_captured(ops):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_coefficients_of_one_image_in_either_shape(ops):
+    x = normal(1, 1, 7, 9, 40).to(torch.bfloat16)
+    a, b, ya, yb = (normal(i, 40) for i in range(2, 6))
+    cw, yw = ops.checkpoint8_write(x, a, b, ya, yb, act="relu")
+    for first in (False, True):
+        one = [t.view(1, 40) if (i < 2) == first else t for i, t in enumerate((a, b, ya, yb))]
+        ck, y = ops.checkpoint8_write(x, *one, act="relu")
+        assert torch.equal(y, yw) and torch.equal(ck.codes, cw.codes)
+    assert torch.equal(ops.checkpoint8_read(cw, a.view(1, 40), b.view(1, 40)), ops.checkpoint8_read(cw, a, b))
