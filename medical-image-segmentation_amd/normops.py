@@ -253,6 +253,8 @@ def group_norm_act_backward(dy, saved, out=None):
     """dx, dgamma and dbeta (float32 (C,)) of `group_norm_act` from the gradient of its result and what it saved.  out: where
     dx goes, a view like dy (dy itself allowed)."""
     lib = L.load()
+    if not isinstance(saved, Saved) or not isinstance(saved.checkpoint, (Checkpoint8, type(None))):
+        raise L.MisegError("the backward pass takes what group_norm_act saved")
     d = L.GroupNormBwdDesc()
     d.dy_pix, d.dy_img = _view(dy, "dy")
     n, h, w, c = dy.shape
@@ -305,7 +307,7 @@ def _pair(a, b, what, n, c, device):
         return None, None, 0
     if a is None or b is None:
         raise L.MisegError("%s: a scale and a shift go together" % what)
-    shape = (n, c) if a.dim() == 2 else (c,)
+    shape = (n, c) if isinstance(a, torch.Tensor) and a.dim() == 2 else (c,)
     _coef(a, what + " scale", shape, device)
     _coef(b, what + " shift", shape, device)
     return _aligned(a), _aligned(b), c if a.dim() == 2 and n > 1 else 0      # of one image both shapes are the same
@@ -334,9 +336,9 @@ def checkpoint8_write(x, scale=None, shift=None, y_scale=None, y_shift=None, act
     y = None
     if y_scale is not None:
         y = x.new_empty((n, h, w, c)) if out is None else out
+        d.y_pix, d.y_img = _view(y, "out", x)
         if y.dtype != x.dtype:
             raise L.MisegError("out is %s, x %s" % (y.dtype, x.dtype))
-        d.y_pix, d.y_img = _view(y, "out", x)
         d.y = y.data_ptr()
     elif out is not None or act != "none":
         raise L.MisegError("an activation and out belong to y, which takes y_scale and y_shift")
@@ -352,6 +354,8 @@ def checkpoint8_write(x, scale=None, shift=None, y_scale=None, y_shift=None, act
 def checkpoint8_read(checkpoint, scale=None, shift=None, act="none", dtype=torch.bfloat16, out=None):
     """act(v * scale + shift) of a checkpoint's values v as a tensor of `dtype` (of out's type where it is given)."""
     lib = L.load()
+    if not isinstance(checkpoint, Checkpoint8):
+        raise L.MisegError("checkpoint8_read takes a Checkpoint8, not %s" % type(checkpoint).__name__)
     codes = checkpoint.codes
     n, h, w, c = codes.shape
     device = codes.device

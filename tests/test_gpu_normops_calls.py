@@ -169,3 +169,27 @@ def test_coefficients_of_one_image_in_either_shape(ops):
         ck, y = ops.checkpoint8_write(x, *one, act="relu")
         assert torch.equal(y, yw) and torch.equal(ck.codes, cw.codes)
     assert torch.equal(ops.checkpoint8_read(cw, a.view(1, 40), b.view(1, 40)), ops.checkpoint8_read(cw, a, b))
+
+
+def test_arguments_of_other_kinds_are_refused(ops):
+    from miseg_amd import lib as L
+    x, g = normal(1, 2, 5, 6, 32), normal(2, 32)
+    ck = ops.checkpoint8_write(x)
+    for out in ("y", 1, [x]):
+        for call in (lambda: ops.group_norm_act(x, g, g, 4, out=out), lambda: ops.checkpoint8_write(x, None, None, g, g, out=out),
+                     lambda: ops.checkpoint8_read(ck, out=out)):
+            with pytest.raises(L.MisegError):
+                call()
+    for bad in (1.0, "a", [1.0] * 32):
+        for call in (lambda: ops.checkpoint8_write(x, bad, g), lambda: ops.checkpoint8_write(x, g, bad),
+                     lambda: ops.checkpoint8_read(ck, bad, g), lambda: ops.checkpoint8_read(ck, g, bad),
+                     lambda: ops.group_norm_act(x, bad, g, 4)):
+            with pytest.raises(L.MisegError):
+                call()
+    for bad in (x, None, (ck.codes, ck.scales)):
+        with pytest.raises(L.MisegError):
+            ops.checkpoint8_read(bad)
+        with pytest.raises(L.MisegError):
+            ops.group_norm_act_backward(x, bad)
+    with pytest.raises(L.MisegError):
+        ops.group_norm_act_backward(x, ops.Saved(None, (ck.codes, ck.scales), g, g, g, g, g, g, 4, "none"))
