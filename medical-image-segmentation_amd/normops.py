@@ -6,8 +6,9 @@ batch statistics only): `group_norm_act` and `group_norm_act_backward` for batch
 
 Tensors are (N, H, W, C) with C a multiple of 8, in bfloat16, float16 or float32, dense or a channel slice of a wider
 dense tensor that starts at a multiple of 16 bytes; empty ones are refused.  Every function launches on the current stream of
-its tensors' device.  There is no autograd behind them: the caller runs the backward pass, as `Trainer` does.  Where autograd
-is recording, a tensor that asks for a gradient is refused: take `.detach()` of it or call under `torch.no_grad()`.
+its tensors' device, through `lib` where one is given (the proxy that times the launches of `Trainer.profile_step`).  There is
+no autograd behind them: the caller runs the backward pass, as `Trainer` does.  Where autograd is recording, a tensor that
+asks for a gradient is refused: take `.detach()` of it or call under `torch.no_grad()`.
 """
 import ctypes as C
 
@@ -204,12 +205,12 @@ def _workspace(lib, d, checkpoint, backward, x):
     return ws
 
 
-def group_norm_act(x, gamma, beta, groups, eps=1e-3, act="none", out=None, checkpoint=False):
+def group_norm_act(x, gamma, beta, groups, eps=1e-3, act="none", out=None, checkpoint=False, lib=None):
     """y = act(gamma * (x - mean) / sqrt(var + eps) + beta), mean and biased variance over the pixels and the C / groups
     consecutive channels of a group of each image.  gamma, beta: float32 (C,) or None (1 and 0).  act: "none", "relu", "silu".
     out: where y goes, a view like x (x itself only with `checkpoint`).  checkpoint: keep the normalised x in 8 bits, not x.
     Returns y and the `Saved` that the backward pass takes."""
-    lib = L.load()
+    lib = L.load() if lib is None else lib
     d = L.GroupNormDesc()
     d.x_pix, d.x_img = _view(x, "x")
     n, h, w, c = x.shape
@@ -249,10 +250,10 @@ def group_norm_act(x, gamma, beta, groups, eps=1e-3, act="none", out=None, check
     return y, Saved._of(None if checkpoint else x, ck, flat, n, c, gamma, beta, groups, act)
 
 
-def group_norm_act_backward(dy, saved, out=None):
+def group_norm_act_backward(dy, saved, out=None, lib=None):
     """dx, dgamma and dbeta (float32 (C,)) of `group_norm_act` from the gradient of its result and what it saved.  out: where
     dx goes, a view like dy (dy itself allowed)."""
-    lib = L.load()
+    lib = L.load() if lib is None else lib
     if not isinstance(saved, Saved) or not isinstance(saved.checkpoint, (Checkpoint8, type(None))):
         raise L.MisegError("the backward pass takes what group_norm_act saved")
     d = L.GroupNormBwdDesc()
@@ -317,10 +318,10 @@ def _pointers(a, b):
     return (None, None) if a is None else (a.data_ptr(), b.data_ptr())
 
 
-def checkpoint8_write(x, scale=None, shift=None, y_scale=None, y_shift=None, act="none", out=None):
+def checkpoint8_write(x, scale=None, shift=None, y_scale=None, y_shift=None, act="none", out=None, lib=None):
     """The 8-bit checkpoint of x, or of x * scale + shift with float32 coefficients (C,) or (N, C).  With y_scale and y_shift
     also y = act(x * y_scale + y_shift) of the same pass, into `out` if given (x itself allowed): returns (checkpoint, y)."""
-    lib = L.load()
+    lib = L.load() if lib is None else lib
     d = L.Checkpoint8Desc()
     d.x_pix, d.x_img = _view(x, "x")
     n, h, w, c = x.shape
@@ -351,9 +352,9 @@ def checkpoint8_write(x, scale=None, shift=None, y_scale=None, y_shift=None, act
     return ck if y is None else (ck, y)
 
 
-def checkpoint8_read(checkpoint, scale=None, shift=None, act="none", dtype=torch.bfloat16, out=None):
+def checkpoint8_read(checkpoint, scale=None, shift=None, act="none", dtype=torch.bfloat16, out=None, lib=None):
     """act(v * scale + shift) of a checkpoint's values v as a tensor of `dtype` (of out's type where it is given)."""
-    lib = L.load()
+    lib = L.load() if lib is None else lib
     if not isinstance(checkpoint, Checkpoint8):
         raise L.MisegError("checkpoint8_read takes a Checkpoint8, not %s" % type(checkpoint).__name__)
     codes = checkpoint.codes

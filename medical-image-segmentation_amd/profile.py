@@ -10,12 +10,45 @@ import collections
 
 import torch
 
+from . import lib as L
+
 
 def _bytes_bn_apply(a):        # x, dy, dx, pixels, C, ..., addend at index 15
     return a[3] * a[4] * 2 * (3 + (1 if a[15] else 0))
 
 
+def _values(d):                # of a normalisation or checkpoint descriptor
+    return d.N * d.pixels * d.C
+
+
+def _type(d):
+    return 4 if d.dtype == L.DT_F32 else 2
+
+
+def _eight(d):                 # their 8-bit checkpoint
+    return _values(d) + 2 * d.N * d.pixels * ((d.C + 31) // 32)
+
+
+def _bytes_group_norm(a):      # x, y and what is kept of it
+    d = a[0]._obj
+    return _values(d) * 2 * _type(d) + (_eight(d) if d.codes else 0)
+
+
+def _bytes_group_norm_bwd(a):  # x or its checkpoint, dy, dx
+    d = a[0]._obj
+    return _values(d) * 2 * _type(d) + (_eight(d) if d.codes else _values(d) * _type(d))
+
+
+def _bytes_checkpoint(a):      # written: x, the checkpoint and y, if any; read: the checkpoint and y
+    d = a[0]._obj
+    return _eight(d) + _values(d) * _type(d) * ((1 if d.x else 0) + (1 if d.y else 0))
+
+
 BYTES = {
+    "miseg_group_norm_act_fwd": _bytes_group_norm,
+    "miseg_group_norm_act_bwd": _bytes_group_norm_bwd,
+    "miseg_checkpoint8_write": _bytes_checkpoint,
+    "miseg_checkpoint8_read": _bytes_checkpoint,
     "miseg_bn_relu_bwd_apply": _bytes_bn_apply,
     "miseg_bn_relu_bwd_reduce": lambda a: a[2] * a[3] * 4,
     "miseg_scale_shift_relu_fwd": lambda a: a[4] * a[5] * 4,
@@ -54,7 +87,8 @@ class TimedLib:
     def __getattr__(self, name):
         fn = getattr(self._lib, name)
         if not self.on or not name.startswith("miseg_") or fn.restype is None or \
-                name in ("miseg_last_error", "miseg_device_check", "miseg_version", "miseg_conv_kernel_name"):
+                name in ("miseg_last_error", "miseg_device_check", "miseg_version", "miseg_conv_kernel_name",
+                        "miseg_group_norm_workspace"):
             return fn
 
         def call(*args):

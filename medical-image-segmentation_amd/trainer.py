@@ -895,7 +895,7 @@ class Trainer:
             return None
         kept = self.kept.get(src)
         if kept is None:
-            kept = self.kept[src] = Kept(normops.checkpoint8_write(xin.t[..., xin.c0:xin.c0 + xin.c]))
+            kept = self.kept[src] = Kept(normops.checkpoint8_write(xin.t[..., xin.c0:xin.c0 + xin.c], lib=self.lib))
         return kept
 
     def _operand(self, kept, side=False):
@@ -906,7 +906,7 @@ class Trainer:
         n, h, w, c = kept.checkpoint.shape
         with torch.cuda.stream(self.side if side else None):
             out = self.new(h, w, c)
-            normops.checkpoint8_read(kept.checkpoint, kept.scale, kept.shift, act=kept.act, out=out.t[..., :c])
+            normops.checkpoint8_read(kept.checkpoint, kept.scale, kept.shift, act=kept.act, out=out.t[..., :c], lib=self.lib)
         return out
 
     def _bn_checkpoint_forward(self, l, relu, xin, s):
@@ -919,7 +919,7 @@ class Trainer:
         beta = self.view(name, "beta")
         out = self.new_out(relu, xin.h, xin.w, c)
         ck, _ = normops.checkpoint8_write(xin.t[..., xin.c0:xin.c0 + c], rstd, -s["mean"][:c] * rstd, s["scale"][:c],
-                                          s["shift"][:c], act="relu", out=out.t[..., out.c0:out.c0 + c])
+                                          s["shift"][:c], act="relu", out=out.t[..., out.c0:out.c0 + c], lib=self.lib)
         self.acts[relu] = out
         self.kept[relu] = Kept(ck, gamma, beta, "relu")
         rows = (1, xin.n * xin.h, xin.w)
@@ -933,7 +933,8 @@ class Trainer:
         rows = (1, dy.n * dy.h, dy.w)
         out = self.new(dy.h, dy.w, c)
         _, dgamma, dbeta = normops.group_norm_act_backward(dy.t.view(*rows, dy.pix)[..., dy.c0:dy.c0 + c],
-                                                           self.saved[name], out=out.t.view(*rows, out.pix)[..., :c])
+                                                           self.saved[name], out=out.t.view(*rows, out.pix)[..., :c],
+                                                           lib=self.lib)
         self.gview(name, "beta").copy_(dbeta)
         if l.config["scale"]:
             self.gview(name, "gamma").copy_(dgamma)

@@ -143,3 +143,32 @@ def test_poolings_and_transpose_convolutions(enc, dec, kind):
                     assert rel(got[a * 2 + b], wt.grad.permute(0, 2, 3, 1)) <= SUMS, (name, a, b)
             seen += 1
     assert seen >= (1 if kind == "pool" else 4), seen
+
+
+def test_a_profiled_step_lists_the_normalisation_and_checkpoint_launches():
+    """Trainer.profile_step times every launch: a checkpoint a BatchNormalization + ReLU and a kept tensor, a read an operand, a
+    backward pass a BatchNormalization, with the bytes they move."""
+    tr, x, gt = make("resnet18", "U-Net", checkpoint_8bit=True)
+    tr.train_step(x, gt)
+    before = tr.P.clone()
+    prof = tr.profile_step(x, gt)
+    assert not torch.equal(tr.P, before)
+    g = tr.g
+    bns = [n for n, l in g.layers.items() if l.cls == "BatchNormalization" and g.layers[l.inbound[0]].cls != "InputLayer"]
+    convs = [n for n, l in g.layers.items() if l.cls in ("Conv2D", "Conv2DTranspose") and l.config["kernel_size"] != 7]
+    pools = [n for n, l in g.layers.items() if l.cls == "MaxPooling2D"]
+    want = {"miseg_checkpoint8_write": len(tr.kept), "miseg_checkpoint8_read": len(convs) + len(pools),
+            "miseg_group_norm_act_bwd": len(bns)}
+    got = {v["entry"]: v for v in prof.values() if v["entry"] in want}
+    assert {k: v["launches"] for k, v in got.items()} == want
+    assert all(v["ms"] > 0 for v in got.values())
+    eight = sum(k.checkpoint.nbytes() for k in tr.kept.values())
+    acts = [2 * k.checkpoint.codes.numel() for k in tr.kept.values()]
+    both = [2 * k.checkpoint.codes.numel() for k in tr.kept.values() if k.scale is not None]
+    assert got["miseg_checkpoint8_write"]["bytes"] == eight + sum(acts) + sum(both)
+    norm = sum(tr.saved[n].checkpoint.nbytes() + 4 * tr.saved[n].checkpoint.codes.numel() for n in bns)
+    assert got["miseg_group_norm_act_bwd"]["bytes"] == norm
+    layers = {tag for tag, kernel, _, _, _ in tr.lib.calls() if "group_norm" in kernel}
+    assert layers == {"bwd " + n for n in bns}
+    tr.train_step(x, gt)                                       # and nothing is recorded afterwards
+    assert len(tr.lib.records) == sum(v["launches"] for v in prof.values())
