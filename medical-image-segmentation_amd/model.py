@@ -101,7 +101,7 @@ class Model:
         self.loss = None
         self.metrics = []
         self.encoder_freeze = False
-        self.checkpoint_8bit = False       # set before the first fit(): activations kept in 8 bits (trainer.Trainer)
+        self.checkpoint_8bit = False       # training keeps activations in 8 bits (trainer.Trainer), from the next step on
         self._engines = {}
         self._storage = "fp16"
 
@@ -303,6 +303,8 @@ class Model:
             # parameters, optimiser state and BatchNorm scratch do not depend on the batch size and
             # activations are allocated per step: a short last batch of a dataset costs nothing
             t.set_batch(batch)
+        if t.checkpoint_8bit != bool(self.checkpoint_8bit):
+            t.set_checkpoint_8bit(self.checkpoint_8bit)
         return t
 
     @property

@@ -127,10 +127,7 @@ class Trainer:
         self.focal = bool(self.loss_flags & L.LOSS_FOCAL)
         self.focal_alpha, self.focal_gamma = LS.FOCAL_ALPHA, LS.FOCAL_GAMMA
         self.world = world_size
-        self.checkpoint_8bit = bool(checkpoint_8bit)
-        if self.checkpoint_8bit and any(l.cls == "Conv2D" and l.config.get("activation") == "relu"
-                                        for l in graph.layers.values()):
-            raise NotImplementedError("8-bit checkpoints of a network whose convolutions have a ReLU of their own")
+        self.checkpoint_8bit = self._can_checkpoint(checkpoint_8bit)
         # encoder_freeze (utils/model.py:179,191,203): the backbone's layers keep their weights and
         # their BatchNormalization layers run on the moving statistics
         self.frozen = set()
@@ -144,6 +141,18 @@ class Trainer:
         self._alloc_params(weights)
         self.keep_grads = False       # debugging: keep (dy, dx) of every layer of the last backward
         self.grad_log = None
+
+    def _can_checkpoint(self, on):
+        if on and any(l.cls == "Conv2D" and l.config.get("activation") == "relu" for l in self.g.layers.values()):
+            raise NotImplementedError("8-bit checkpoints of a network whose convolutions have a ReLU of their own")
+        return bool(on)
+
+    def set_checkpoint_8bit(self, on):
+        """8-bit checkpoints from the next step on, or 16-bit activations again; parameters and optimiser state stay."""
+        self.checkpoint_8bit = self._can_checkpoint(on)
+        self._analyse()
+        self._dgrad_cache = {}            # the folded forms keep weights of their own under their layers' names
+        self.saved, self.kept, self.acts = {}, {}, {}       # a forward pass of the other form has no backward pass here
 
     # ------------------------------------------------------------------ graph analysis
     def _analyse(self):

@@ -172,3 +172,36 @@ def test_a_profiled_step_lists_the_normalisation_and_checkpoint_launches():
     assert layers == {"bwd " + n for n in bns}
     tr.train_step(x, gt)                                       # and nothing is recorded afterwards
     assert len(tr.lib.records) == sum(v["launches"] for v in prof.values())
+
+
+def test_the_choice_may_change_between_steps():
+    """model.checkpoint_8bit counts when it is set: the next step keeps 8 bits, with the parameters and the optimiser's state of
+    the steps before, and one that cannot is refused before anything changes."""
+    from utils.model import make_model, CUSTOM_OBJECTS, METRICS
+    rng = np.random.default_rng(0)
+    x = rng.random((2, 64, 96, 3), dtype=np.float32)
+    y = np.eye(3, dtype=np.float32)[rng.integers(0, 3, (2, 64, 96))]
+    for dec in ("U-Net", "FPN"):
+        model = make_model("resnet18", dec, (64, 96, 3), 3, 1e-3, CUSTOM_OBJECTS["categorical_crossentropy_plus_dice_loss"],
+                           METRICS, False, "m")
+        model.train_on_batch(x, y)
+        tr = model._train_state
+        assert not tr.checkpoint_8bit and not tr.drops
+        for on in (True, False, True):
+            model.checkpoint_8bit = on
+            before = tr.P.clone()
+            model.train_on_batch(x, y)
+            assert model._train_state is tr and tr.checkpoint_8bit == on and bool(tr.kept) == on
+            assert not torch.equal(tr.P, before)
+        assert tr.step_count == 4
+        # the folded forms of a network are those of a trainer that never kept 8 bits
+        fresh, _, _ = make("resnet18", dec)
+        tr.set_checkpoint_8bit(False)
+        assert (tr.head_up, tr.fs, tr.p2, tr.place) == (fresh.head_up, fresh.fs, fresh.p2, fresh.place)
+        fresh.load_state(tr.state())
+        xt, gt = torch.from_numpy(x).cuda(), torch.from_numpy(y).cuda()
+        assert rel(tr.forward(xt), fresh.forward(xt)) <= 20 ** 0.5 * BF      # twenty layers' roundings of random sign
+    tr, _, _ = make("vgg16", "U-Net")
+    with pytest.raises(NotImplementedError):
+        tr.set_checkpoint_8bit(True)
+    assert not tr.checkpoint_8bit
