@@ -1324,6 +1324,12 @@ static SmallGrid small_grid(long long N, long long pixels, int C, int groups, bo
   return g;
 }
 
+// Images that one launch of the small form takes: at most 2^32 threads in a direction of a grid.
+static int small_images(const SmallGrid& g) {
+  const long long n = ((1LL << 32) - 1) / g.threads / g.slabs;
+  return (int)(n < 65535 ? n : 65535);
+}
+
 // Partial sums of a group that one block adds up (10 thousand: 7 us, as the chip); more are left to the whole chip.
 constexpr int kWidePartials = 16384;
 
@@ -1413,21 +1419,31 @@ int launch_group_norm_fwd(const miseg_group_norm_desc* d, hipStream_t s) {
   const NormParams param{d->gamma, d->beta, d->gamma_kept, d->beta_kept};
   const SmallGrid sg = small_fwd(d->N, d->pixels, d->C, d->groups, d->dtype, d->codes != nullptr);
   if (sg.threads) {
-    SmallFwdArgs p{(const char*)d->x, (char*)d->y, (signed char*)d->codes, (bf16_t*)d->code_scales, param,
-                   d->mean, d->rstd, d->scale, d->shift, d->x_pix, d->x_img, d->y_pix, d->y_img, (int)d->pixels, d->C,
-                   d->groups, act_of(d->act), d->N * sg.slabs, d->eps, sg};
-    const dim3 grid(p.blocks), block(sg.threads);
-    by_type_act(storage, NA_NONE, [&](auto t, auto) {
-      typedef decltype(t) T;
-      typedef SmallHold<T> H;
-      if (sg.threads == kSmallThreads[0]) {
-        if (d->codes) hipLaunchKernelGGL((gn_small_fwd_kernel<T, true, kSmallThreads[0], H::fwd[0]>), grid, block, 0, s, p);
-        else hipLaunchKernelGGL((gn_small_fwd_kernel<T, false, kSmallThreads[0], H::fwd[0]>), grid, block, 0, s, p);
-      } else {
-        if (d->codes) hipLaunchKernelGGL((gn_small_fwd_kernel<T, true, kSmallThreads[1], H::fwd[1]>), grid, block, 0, s, p);
-        else hipLaunchKernelGGL((gn_small_fwd_kernel<T, false, kSmallThreads[1], H::fwd[1]>), grid, block, 0, s, p);
+    const int most = small_images(sg);
+    for (int n0 = 0; n0 < d->N; n0 += most) {
+      const int n = d->N - n0 < most ? d->N - n0 : most;
+      const long long cat = (long long)n0 * d->C, gat = (long long)n0 * d->groups;
+      SmallFwdArgs p{(const char*)d->x + n0 * d->x_img * bytes, (char*)d->y + n0 * d->y_img * bytes, (signed char*)d->codes,
+                     (bf16_t*)d->code_scales, n0 ? NormParams{d->gamma, d->beta, nullptr, nullptr} : param, d->mean + gat,
+                     d->rstd + gat, d->scale + cat, d->shift + cat, d->x_pix, d->x_img, d->y_pix, d->y_img, (int)d->pixels,
+                     d->C, d->groups, act_of(d->act), n * sg.slabs, d->eps, sg};
+      if (p.codes) {
+        p.codes += n0 * d->pixels * d->C;
+        p.scales += n0 * d->pixels * ((d->C + 31) / 32);
       }
-    });
+      const dim3 grid(p.blocks), block(sg.threads);
+      by_type_act(storage, NA_NONE, [&](auto t, auto) {
+        typedef decltype(t) T;
+        typedef SmallHold<T> H;
+        if (sg.threads == kSmallThreads[0]) {
+          if (d->codes) hipLaunchKernelGGL((gn_small_fwd_kernel<T, true, kSmallThreads[0], H::fwd[0]>), grid, block, 0, s, p);
+          else hipLaunchKernelGGL((gn_small_fwd_kernel<T, false, kSmallThreads[0], H::fwd[0]>), grid, block, 0, s, p);
+        } else {
+          if (d->codes) hipLaunchKernelGGL((gn_small_fwd_kernel<T, true, kSmallThreads[1], H::fwd[1]>), grid, block, 0, s, p);
+          else hipLaunchKernelGGL((gn_small_fwd_kernel<T, false, kSmallThreads[1], H::fwd[1]>), grid, block, 0, s, p);
+        }
+      });
+    }
     MISEG_CHECK_HIP(hipGetLastError());
     return MISEG_OK;
   }
@@ -1505,23 +1521,33 @@ int launch_group_norm_bwd(const miseg_group_norm_bwd_desc* d, hipStream_t s) {
   double2* sums = (double2*)ws;
   const SmallGrid sg = small_bwd(d->N, d->pixels, d->C, d->groups, d->dtype);
   if (sg.threads) {
-    SmallBwdArgs q{{(const char*)d->x, (const char*)d->dy, (char*)d->dx, (const signed char*)d->codes,
-                    (const bf16_t*)d->code_scales, d->mean, d->rstd, d->scale, d->shift, d->gamma, d->beta, nullptr, nullptr,
-                    nullptr, nullptr, nullptr, d->dgamma, d->dbeta, d->x_pix, d->x_img, d->dy_pix, d->dy_img, d->dx_pix,
-                    d->dx_img, (int)d->pixels, d->C, d->groups, d->N, NormGrid{}, nullptr, nullptr, 0},
-                   sums, act, d->N * sg.slabs, sg};
-    const dim3 grid(q.blocks), block(sg.threads);
-    by_type_act(storage, NA_NONE, [&](auto t, auto) {
-      typedef decltype(t) T;
-      typedef SmallHold<T> H;
-      if (sg.threads == kSmallBack[0]) {
-        if (ck) hipLaunchKernelGGL((gn_small_bwd_kernel<T, true, kSmallBack[0], H::bwd[0]>), grid, block, 0, s, q);
-        else hipLaunchKernelGGL((gn_small_bwd_kernel<T, false, kSmallBack[0], H::bwd[0]>), grid, block, 0, s, q);
-      } else {
-        if (ck) hipLaunchKernelGGL((gn_small_bwd_kernel<T, true, kSmallBack[1], H::bwd[1]>), grid, block, 0, s, q);
-        else hipLaunchKernelGGL((gn_small_bwd_kernel<T, false, kSmallBack[1], H::bwd[1]>), grid, block, 0, s, q);
+    const int most = small_images(sg);
+    for (int n0 = 0; n0 < d->N; n0 += most) {
+      const int n = d->N - n0 < most ? d->N - n0 : most;
+      const long long cat = (long long)n0 * d->C, gat = (long long)n0 * d->groups;
+      SmallBwdArgs q{{(const char*)d->x + n0 * d->x_img * bytes, (const char*)d->dy + n0 * d->dy_img * bytes,
+                      (char*)d->dx + n0 * d->dx_img * bytes, (const signed char*)d->codes, (const bf16_t*)d->code_scales,
+                      d->mean + gat, d->rstd + gat, d->scale + cat, d->shift + cat, d->gamma, d->beta, nullptr, nullptr,
+                      nullptr, nullptr, nullptr, d->dgamma, d->dbeta, d->x_pix, d->x_img, d->dy_pix, d->dy_img, d->dx_pix,
+                      d->dx_img, (int)d->pixels, d->C, d->groups, d->N, NormGrid{}, nullptr, nullptr, 0},
+                     sums + cat, act, n * sg.slabs, sg};
+      if (ck) {
+        q.p.codes += n0 * d->pixels * d->C;
+        q.p.scales += n0 * d->pixels * ((d->C + 31) / 32);
       }
-    });
+      const dim3 grid(q.blocks), block(sg.threads);
+      by_type_act(storage, NA_NONE, [&](auto t, auto) {
+        typedef decltype(t) T;
+        typedef SmallHold<T> H;
+        if (sg.threads == kSmallBack[0]) {
+          if (ck) hipLaunchKernelGGL((gn_small_bwd_kernel<T, true, kSmallBack[0], H::bwd[0]>), grid, block, 0, s, q);
+          else hipLaunchKernelGGL((gn_small_bwd_kernel<T, false, kSmallBack[0], H::bwd[0]>), grid, block, 0, s, q);
+        } else {
+          if (ck) hipLaunchKernelGGL((gn_small_bwd_kernel<T, true, kSmallBack[1], H::bwd[1]>), grid, block, 0, s, q);
+          else hipLaunchKernelGGL((gn_small_bwd_kernel<T, false, kSmallBack[1], H::bwd[1]>), grid, block, 0, s, q);
+        }
+      });
+    }
     if (d->N > 1 && (d->dgamma || d->dbeta))
       hipLaunchKernelGGL(gn_bwd_params_kernel, dim3((d->C + kParamChannels - 1) / kParamChannels), dim3(kNormThreads), 0, s, sums,
                          d->N, d->C, d->dgamma, d->dbeta);

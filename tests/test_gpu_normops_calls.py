@@ -193,3 +193,42 @@ def test_arguments_of_other_kinds_are_refused(ops):
             ops.group_norm_act_backward(x, bad)
     with pytest.raises(L.MisegError):
         ops.group_norm_act_backward(x, ops.Saved(None, (ck.codes, ck.scales), g, g, g, g, g, g, 4, "none"))
+
+
+@pytest.mark.parametrize("checkpoint", [False, True])
+def test_more_small_blocks_than_a_launch_takes(ops, checkpoint):
+    """65535 images of one pixel in 257 slabs of 40 channels: 16.8 million blocks of 256 threads, and a launch takes 2^32
+    threads at most in a direction.  Images are apart, so the last ones give what a call of their own gives."""
+    n, c, groups = 65535, 10280, 257
+    x = torch.empty((n, 1, 1, c), dtype=torch.bfloat16, device="cuda")
+    for i in range(0, n, 8192):
+        m = min(8192, n - i)
+        x[i:i + m] = normal(i, m, 1, 1, c)
+    gamma, beta = normal(1, c), normal(2, c)
+    dy = x.flip(0)
+    y, saved = ops.group_norm_act(x, gamma, beta, groups, act="relu", checkpoint=checkpoint)
+    dx, dgamma, dbeta = ops.group_norm_act_backward(dy, saved)
+    sums = torch.zeros((2, c), dtype=torch.float64, device="cuda")
+    size = torch.zeros((2, c), dtype=torch.float64, device="cuda")
+    for i in range(0, n, 4096):
+        part = slice(i, min(i + 4096, n))
+        yw, sw = ops.group_norm_act(x[part], gamma, beta, groups, act="relu", checkpoint=checkpoint)
+        dxw, _, _ = ops.group_norm_act_backward(dy[part], sw)
+        assert torch.equal(y[part], yw) and torch.equal(dx[part], dxw), i
+        assert torch.equal(saved.mean[part], sw.mean) and torch.equal(saved.shift[part], sw.shift)
+        if checkpoint:
+            assert torch.equal(saved.checkpoint.codes[part], sw.checkpoint.codes)
+            xhat = sw.checkpoint.codes.double() * sw.checkpoint.scales.double().repeat_interleave(32, 3)[..., :c]
+            z = xhat * gamma.double() + beta.double()
+        else:
+            xhat = (x[part].double() - sw.mean.double().repeat_interleave(40, 1)[:, None, None]) * \
+                sw.rstd.double().repeat_interleave(40, 1)[:, None, None]
+            z = x[part].double() * sw.scale.double()[:, None, None] + sw.shift.double()[:, None, None]
+        g = dy[part].double() * (z > 0)
+        for k, t in enumerate((g * xhat, g)):
+            sums[k] += t.sum((0, 1, 2))
+            size[k] += t.abs().sum((0, 1, 2))
+    # an image's term a channel is one product of 32-bit numbers (x - mean, rstd, g: 4 roundings), images are added up in 64
+    # bits and the sum is rounded once
+    for k, got in enumerate((dgamma, dbeta)):
+        assert ((got.double() - sums[k]).abs() <= 4 * U * size[k] + U * sums[k].abs()).all()
