@@ -120,11 +120,12 @@ class Saved:
                      zip(self._four, ("mean", "rstd", "scale", "shift"), ((n, g), (n, g), (n, c), (n, c))))
 
     def _parameters(self, n, c, device):
-        """Addresses of gamma and beta, or None; after `_addresses`."""
-        own = self.__dict__
-        at = self._flat.data_ptr() + 8 * n * c if "gamma" not in own or "beta" not in own else 0
-        return _coef(self.gamma, "gamma", (c,), device) if "gamma" in own else at, \
-            _coef(self.beta, "beta", (c,), device) if "beta" in own else at + 4 * c
+        """Addresses of gamma and beta, or None, for the pass from a checkpoint; after `_addresses`."""
+        own = self.__dict__.get
+        gamma, beta = own("gamma", self), own("beta", self)      # self: in the buffer
+        at = self._flat.data_ptr() + 8 * n * c if gamma is self or beta is self else 0
+        return at if gamma is self else _coef(gamma, "gamma", (c,), device), \
+            at + 4 * c if beta is self else _coef(beta, "beta", (c,), device)
 
 
 def _view(t, name, like=None):
@@ -136,7 +137,7 @@ def _view(t, name, like=None):
     if like is not None and (t.shape != like.shape or t.device != like.device):
         raise L.MisegError("%s is %s on %s, not %s on %s" % (name, tuple(t.shape), t.device, tuple(like.shape), like.device))
     n, h, w, c = t.shape
-    if t.numel() == 0:
+    if not (n and h and w and c):
         raise L.MisegError("%s is empty: %s" % (name, tuple(t.shape)))
     if n > 65535 or c > 65536:                               # before the 32 bits of a descriptor cut them
         raise L.MisegError("%s: %d images of %d channels (at most 65535 of 65536)" % (name, n, c))
@@ -162,12 +163,12 @@ def _coef(t, name, shape, device, optional=True):
     return t.data_ptr()
 
 
-def _plain(*tensors):
+def _plain(a, b=None, c=None):
     """Nothing that autograd would have to see."""
-    for t in tensors:
-        if t is not None and t.requires_grad and torch.is_grad_enabled():
-            raise L.MisegError("a tensor asks for a gradient, and no autograd is behind this call: detach it or call under "
-                               "torch.no_grad()")
+    if (a is not None and a.requires_grad or b is not None and b.requires_grad or c is not None and c.requires_grad) and \
+            torch.is_grad_enabled():
+        raise L.MisegError("a tensor asks for a gradient, and no autograd is behind this call: detach it or call under "
+                           "torch.no_grad()")
 
 
 def _act(act):
@@ -194,8 +195,8 @@ def _launch(fn, d, device):
         L.check(rc)
 
 
-def _workspace(lib, d, checkpoint, backward, x):
-    size = lib.miseg_group_norm_workspace(d.N, d.pixels, d.C, d.groups, d.dtype, checkpoint, backward)
+def _workspace(lib, d, n, pixels, c, groups, dtype, checkpoint, backward, x):
+    size = lib.miseg_group_norm_workspace(n, pixels, c, groups, dtype, checkpoint, backward)
     if size < 0:
         L.check(int(size))
     if size == 0:
@@ -227,9 +228,10 @@ def group_norm_act(x, gamma, beta, groups, eps=1e-3, act="none", out=None, check
             raise L.MisegError("out is %s, x %s" % (y.dtype, dtype))
         if y.data_ptr() == d.x and not checkpoint:
             raise L.MisegError("out is x, which the backward pass needs: pass checkpoint=True or another tensor")
+        _plain(y)
     d.y = y.data_ptr()
     d.gamma, d.beta = _coef(gamma, "gamma", (c,), device), _coef(beta, "beta", (c,), device)
-    _plain(x, gamma, beta, out)
+    _plain(x, gamma, beta)
     flat = x.new_empty(2 * (n * (c + groups) + (c if checkpoint else 0)), dtype=torch.float32)
     d.scale = at = flat.data_ptr()
     d.shift, stats = at + 4 * n * c, at + 8 * n * c
@@ -244,8 +246,9 @@ def group_norm_act(x, gamma, beta, groups, eps=1e-3, act="none", out=None, check
         d.codes, d.code_scales = ck.codes.data_ptr(), ck.scales.data_ptr()
     d.mean, d.rstd = stats, stats + 4 * n * groups
     d.N, d.C, d.groups, d.pixels, d.eps, d.act = n, c, groups, h * w, eps, _act(act)
-    d.dtype, d.fmt = _TYPES[dtype]
-    ws = _workspace(lib, d, 1 if checkpoint else 0, 0, x)    # noqa: F841: lives until the launch is in its stream
+    d.dtype, d.fmt = kind = _TYPES[dtype]
+    # the workspace lives until the launch is in its stream
+    ws = _workspace(lib, d, n, h * w, c, groups, kind[0], 1 if checkpoint else 0, 0, x)      # noqa: F841
     _launch(lib.miseg_group_norm_act_fwd, d, device)
     return y, Saved._of(None if checkpoint else x, ck, flat, n, c, gamma, beta, groups, act)
 
@@ -284,38 +287,34 @@ def group_norm_act_backward(dy, saved, out=None, lib=None):
     _plain(dy, out)
     d.dx = dx.data_ptr()
     d.mean, d.rstd, d.scale, d.shift = saved._addresses(n, c, device)
-    d.gamma, d.beta = saved._parameters(n, c, device)
+    if ck is not None:
+        d.gamma, d.beta = saved._parameters(n, c, device)
     grads = dy.new_empty((2, c), dtype=torch.float32)
     d.dgamma = at = grads.data_ptr()
     d.dbeta = at + 4 * c
     d.N, d.C, d.groups, d.pixels, d.act = n, c, groups, h * w, _act(saved.act)
-    d.dtype, d.fmt = _TYPES[dtype]
-    ws = _workspace(lib, d, 0 if ck is None else 1, 1, dy)   # noqa: F841
+    d.dtype, d.fmt = kind = _TYPES[dtype]
+    ws = _workspace(lib, d, n, h * w, c, groups, kind[0], 0 if ck is None else 1, 1, dy)     # noqa: F841
     _launch(lib.miseg_group_norm_act_bwd, d, device)
     dgamma, dbeta = grads.unbind(0)
     return dx, dgamma, dbeta
 
 
-def _aligned(t):
-    """t, or a copy of it at a multiple of 16 bytes: a slice of a flat buffer need not start at one."""
-    return t if t.data_ptr() & 15 == 0 else t.clone()
-
-
 def _pair(a, b, what, n, c, device):
-    """Coefficients (C,) or (N, C) as (tensor, tensor, elements from one image's to the next's); the caller holds them until
-    the launch is in its stream."""
+    """Coefficients (C,) or (N, C) as (pointer, pointer, elements from one image's to the next's, what the caller holds until
+    the launch is in its stream)."""
     if a is None and b is None:
-        return None, None, 0
+        return None, None, 0, None
     if a is None or b is None:
         raise L.MisegError("%s: a scale and a shift go together" % what)
     shape = (n, c) if isinstance(a, torch.Tensor) and a.dim() == 2 else (c,)
-    _coef(a, what + " scale", shape, device)
-    _coef(b, what + " shift", shape, device)
-    return _aligned(a), _aligned(b), c if a.dim() == 2 and n > 1 else 0      # of one image both shapes are the same
-
-
-def _pointers(a, b):
-    return (None, None) if a is None else (a.data_ptr(), b.data_ptr())
+    pa, pb = _coef(a, what + " scale", shape, device), _coef(b, what + " shift", shape, device)
+    _plain(a, b)
+    held = None
+    if (pa | pb) & 15:                                       # slices of a flat buffer: copies start at a multiple of 16 bytes
+        held = a.clone(), b.clone()
+        pa, pb = held[0].data_ptr(), held[1].data_ptr()
+    return pa, pb, c if n > 1 and len(shape) == 2 else 0, held               # of one image both shapes are the same
 
 
 def checkpoint8_write(x, scale=None, shift=None, y_scale=None, y_shift=None, act="none", out=None, lib=None):
@@ -327,10 +326,8 @@ def checkpoint8_write(x, scale=None, shift=None, y_scale=None, y_shift=None, act
     n, h, w, c = x.shape
     device = x.device
     d.x = x.data_ptr()
-    scale, shift, img = _pair(scale, shift, "code", n, c, device)
-    y_scale, y_shift, y_of = _pair(y_scale, y_shift, "y", n, c, device)
-    d.code_a, d.code_b = _pointers(scale, shift)
-    d.y_a, d.y_b = _pointers(y_scale, y_shift)
+    d.code_a, d.code_b, img, held = _pair(scale, shift, "code", n, c, device)                # noqa: F841
+    d.y_a, d.y_b, y_of, y_held = _pair(y_scale, y_shift, "y", n, c, device)                  # noqa: F841
     if scale is not None and y_scale is not None and img != y_of:
         raise L.MisegError("the coefficients of the codes and of y are both (C,) or both (N, C)")
     d.coef_img = max(img, y_of)
@@ -343,7 +340,7 @@ def checkpoint8_write(x, scale=None, shift=None, y_scale=None, y_shift=None, act
         d.y = y.data_ptr()
     elif out is not None or act != "none":
         raise L.MisegError("an activation and out belong to y, which takes y_scale and y_shift")
-    _plain(x, scale, shift, y_scale, y_shift, out)
+    _plain(x, out)
     ck = Checkpoint8._like(x)
     d.codes, d.code_scales = ck.codes.data_ptr(), ck.scales.data_ptr()
     d.N, d.C, d.pixels, d.act = n, c, h * w, _act(act)
@@ -365,9 +362,8 @@ def checkpoint8_read(checkpoint, scale=None, shift=None, act="none", dtype=torch
     d = L.Checkpoint8Desc()
     d.y_pix, d.y_img = _view(out, "out", checkpoint)
     d.y, d.codes, d.code_scales = out.data_ptr(), codes.data_ptr(), checkpoint.scales.data_ptr()
-    scale, shift, d.coef_img = _pair(scale, shift, "y", n, c, device)
-    d.y_a, d.y_b = _pointers(scale, shift)
-    _plain(scale, shift, out)
+    _plain(out)
+    d.y_a, d.y_b, d.coef_img, held = _pair(scale, shift, "y", n, c, device)                  # noqa: F841
     d.N, d.C, d.pixels, d.act = n, c, h * w, _act(act)
     d.dtype, d.fmt = _TYPES[out.dtype]
     _launch(lib.miseg_checkpoint8_read, d, device)
