@@ -36,7 +36,7 @@ def close(got, want, tol):
 SHAPES = [(2, 40, 50, 64, 8), (3, 61, 83, 40, 5), (1, 90, 80, 72, 9), (1, 960, 1280, 64, 16), (2, 75, 80, 1560, 3), (6, 480, 640, 64, 1)]
 
 
-def check(x, groups, saved, extra):
+def check(x, groups, saved, extra, K=K):
     n, h, w, c = x.shape
     for i in range(n):                                         # an image at a time: the reference is in 64 bits
         v = x[i].double().reshape(h * w, groups, c // groups)
@@ -71,3 +71,33 @@ def test_a_first_pixel_far_from_the_rest(ops, shape, offset, dt):
     x = x.to(dt)
     _, saved = ops.group_norm_act(x, None, None, groups, eps=0.0)
     check(x, groups, saved, lambda std: 1.5 * U * N * N * offset * offset / (h * w * std * std))
+
+
+# more terms a thread than the 64 that a K of 160 covers at the worst: pixels of a block over pixels of a sweep
+LONG = [((1, 1920, 1280, 48, 6), 115), ((2, 300, 400, 1032, 43), 142), ((1, 3, 700, 65536, 1), 132), ((5, 480, 640, 64, 16), 95)]
+
+
+@pytest.mark.parametrize("checkpoint", [False, True])
+@pytest.mark.parametrize("shape,terms", LONG, ids=str)
+def test_sums_of_many_terms_a_thread(ops, shape, terms, checkpoint):
+    """Statistics within 1.5 of their own number of terms (and 32 roundings) of u; the parameters' gradients within that number
+    and the 8 roundings of a term (g, x - mean, their product, rstd; mean and rstd are the call's own) of their magnitudes."""
+    n, h, w, c, groups = shape
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    x = (torch.randn((n, h, w, c), generator=gen, device="cuda") + 1).to(torch.bfloat16)
+    dy = torch.randn((n, h, w, c), generator=gen, device="cuda").to(torch.bfloat16)
+    _, saved = ops.group_norm_act(x, None, None, groups, eps=0.0, checkpoint=checkpoint)
+    check(x, groups, saved, lambda std: 0.0, 1.5 * terms + 32)
+    _, dgamma, dbeta = ops.group_norm_act_backward(dy, saved)
+    sums = torch.zeros((4, c), dtype=torch.float64, device="cuda")
+    for i in range(n):
+        g = dy[i].double()
+        if checkpoint:
+            ck = saved.checkpoint
+            xhat = ck.codes[i].double() * ck.scales[i].double().repeat_interleave(32, 2)[..., :c]
+        else:
+            xhat = (x[i].double() - saved.mean[i].double().repeat_interleave(c // groups)) * \
+                saved.rstd[i].double().repeat_interleave(c // groups)
+        sums += torch.stack([t.sum((0, 1)) for t in (g * xhat, g, (g * xhat).abs(), g.abs())])
+    close(dgamma, sums[0], (terms + 8) * U * sums[2])
+    close(dbeta, sums[1], (terms + 8) * U * sums[3])
