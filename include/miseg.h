@@ -615,7 +615,9 @@ int miseg_group_norm_act_bwd(const miseg_group_norm_bwd_desc* d, void* stream);
 /*
  * Activation checkpoints in 8 bits: codes int8 [N * pixels][C], code_scales bf16 [N * pixels][ceil(C / 32)], dense.  32
  * consecutive channels of a pixel share code_scale = bf16(max |v| / 127); v is read back as code * code_scale.  A block
- * whose largest magnitude is below 2^-119 is zero; a block that holds an infinity or a NaN reads back as NaN.
+ * whose largest magnitude is below 2^-119 is zero; a block that holds an infinity or a NaN reads back as NaN.  v is read back
+ * within half a step, code_scale / 2, and rounded to y's type: a magnitude that close to the type's largest may become an
+ * infinity (65504 in fp16 does).
  * Write: v = x * code_a[c] + code_b[c], or x where code_a is NULL; with y also y = act(x * y_a[c] + y_b[c]) in the same
  * pass (a normalisation layer's apply pass that leaves its checkpoint behind).
  * Read: y = act(v * y_a[c] + y_b[c]), or act(v) where y_a is NULL: the operand of a weight gradient.

@@ -180,8 +180,8 @@ struct NormParams {
 };
 
 // ---- the 8-bit block format: 32 consecutive channels of a pixel share a bf16 scale, bf16(amax / 127).
-// code = rint(v / scale): |code| <= 127 because the scale's rounding moves amax / scale by at most 2^-9 of 127, less than
-// half a step.  Below 2^-119 the scale would be a subnormal number and its reciprocal infinite: such a block is zero.  A
+// code = rint(v / scale): |code| <= 127 because the scale's rounding moves amax / scale by at most 2^-8 of 127, to 127.496,
+// less than half a step.  Below 2^-119 the scale would be a subnormal number and its reciprocal infinite: such a block is zero.  A
 // value that is not finite makes the scale NaN, so that all of its block reads back as NaN and an overflow is not lost.
 struct Quant8 { uint2 codes; bf16_t scale; };
 // The definition's operations are single 32-bit roundings: m / 127 and 1 / scale, here by a reciprocal and a correction

@@ -170,8 +170,8 @@ struct GroupCuts {
 // ------------------------------------------------------------------------------------------------ forward statistics
 // Per block and channel: mean and sum of squared differences from it.  A thread sums (x - k) and (x - k)^2 with k its own
 // first value, so that an offset of the channel that is large against its spread does not cancel; threads and blocks are
-// joined by counts, means and sums of squares, a partial a group of the slab (a channel each where slabs cut groups: the
-// finalisation of 120 x 160 x 1536 in one group took 294 us, 6 so).
+// joined by counts, means and sums of squares, a partial a group of the slab, also where slabs cut groups (120 x 160 x 1536 in
+// one group: the finalisation takes 6 us; with a partial a channel it takes 294).
 // Bound by reading x: 157 MB in 30 us (5.3 TB/s).  512 blocks, two a CU, read as fast as 2048 and leave a quarter of the
 // partials: the finalisation of 960 x 1280 x 64 takes 4.9 us, 17 with 2048.
 template <typename T>
@@ -1281,7 +1281,7 @@ static bool good_view(const void* p, int pix, long long img, long long N, long l
 static bool good_coef(const void* p) { return ((uintptr_t)p & 15) == 0; }
 static int bytes_of(int dtype) { return dtype == MISEG_DT_F32 ? 4 : 2; }
 
-constexpr int kStatBlocks = 512, kStatLeast = 8;   // blocks of a reduction, sweeps in the smallest of them
+constexpr int kStatBlocks = 512, kStatLeast = 8;   // blocks of a reduction, sweeps in the smallest of them (4, 16: the same)
 constexpr int kPassBlocks = 32768, kPassLeast = 4; // the same for a pass that only streams
 // Images are taken one launch after the other in steps whose tensors stay in the memory-side cache (256 MB) from the first
 // pass to the second.
@@ -1295,9 +1295,13 @@ template <> struct SmallHold<f32s> { static constexpr int fwd[2] = {4, 8}, bwd[2
 static int gcd_int(int a, int b) { return b ? gcd_int(b, a % b) : a; }
 
 // One launch pays where few pixels meet few channels: a load of a slab narrower than a line keeps a lane for every line, so
-// a block's time grows with its pixels (fp32, 3 x 61 x 83 x 40 in slabs of 8: 17 us in one launch, 10 in two; bf16, 2 x 30 x
-// 40 x 512 backward: 11 us, 15 in three).  Slabs are the widest of whole groups and whole 8s (32s where 32-channel blocks are
-// written) that a block can hold, up to 64 channels, while 256 blocks are left.
+// a block's time grows with its pixels (fp32, 3 x 61 x 83 x 40 in slabs of 8: 17 us in one launch, 10 in two).  bf16, calls in a
+// replayed graph, one launch | the better of two and three: forward 1..8 x 15 x 20 x 512 5.2 to 5.5 us | 9.2 to 10.5, 1..8 x 32 x
+// 64 x 64 6.9 to 7.4 | 8.4 to 9.1, 1..8 x 32 x 64 x 512 8.9 to 13.3 | 11.9 to 16.8; backward with the launch that adds up the
+// parameters, 2 x 30 x 40 x 512 11.9 | 12.5, 8 x 30 x 40 x 512 14.9 | 19.8, 1 x 30 x 40 x 64 8.5 | 9.2.  It loses on narrow maps
+// of many pixels, backward with several images (2 x 30 x 40 x 64 10.8 | 9.4) and forward with a checkpoint (1 x 20 x 30 x 64 10.5 |
+// 9.1, 1 x 32 x 64 x 64 16.1 | 9.3), where a launch less for the host stands against it.  Slabs are the widest of whole groups
+// and whole 8s (32s where 32-channel blocks are written) that a block can hold, up to 64 channels, while 256 blocks are left.
 constexpr int kSmallPixels = 2048;
 static SmallGrid small_grid(long long N, long long pixels, int C, int groups, bool whole32, const int (&threads)[2],
                             const int (&hold)[2]) {
@@ -1339,8 +1343,11 @@ static int images_per_step(long long N, long long image_bytes) {
 }
 
 // Whether an image's partial sums are few enough for every block of the second pass to add them up itself: 4096 of them
-// (32 KB), from blocks that read at most 128 KB of x each.  Two launches and no idle gap for three: 3 x 61 x 83 x 72 out of 8
-// bits 13 us on the GPU, 18 in three.
+// (32 KB), from blocks that read at most 128 KB of x each.  Two launches with a gap between them for three; in a replayed graph
+// 3 x 61 x 83 x 72 forward 10 us (three launches: 11.5), out of 8 bits 10.5 (13.1).  Upwards of 2 x 60 x 80 x 256 (forward 14.1 us,
+// 11.9) and 240 x 320 x 64 (17.1, 14.1; backward the same) three launches are shorter on the GPU and 3.6 us longer on the host.
+// With 64 KB a block 120 x 160 x 256 would take three (14.1 us for 17.8), with 256 KB nothing here changes.  Passes of 512 blocks:
+// 4 x 120 x 160 x 128 with a checkpoint 28.6 us (25.9); of 2048: its backward out of 8 bits 28.6 (26.1).
 constexpr int kFewEntries = 4096, kFewBlocks = 512, kFewPass = 1024;
 constexpr long long kFewBytes = 128 << 10;
 static bool few_partials(long long N, long long pixels, int C, int groups, int bytes, NormGrid& g) {
