@@ -40,8 +40,8 @@ def check(x, groups, saved, extra, K=K):
     n, h, w, c = x.shape
     for i in range(n):                                         # an image at a time: the reference is in 64 bits
         v = x[i].double().reshape(h * w, groups, c // groups)
-        mean = v.mean((0, 2))
-        std = (v - mean[:, None]).square().mean((0, 2)).sqrt()
+        mean = v.mean(2).mean(0)                               # a dimension at a time: torch's means over two of them
+        std = (v - mean[:, None]).square().mean(2).mean(0).sqrt()    # differ from call to call where few values are long sums
         close(saved.mean[i], mean, 4 * U * mean.abs() + K * U * std)
         off = U * mean.abs() / std
         close(saved.rstd[i], 1 / std, (K * U + 4 * off * off + 16 * off / (h * w * c / groups) ** 0.5 + extra(std)) / std)
